@@ -40,6 +40,7 @@ EXPORTS = (
     "arc_fill_causal_mask", "arc_fill_causal_mask_with_block_ids", "arc_qkv_prepare", "arc_sdpa_device_status", "arc_sdpa_clear_device_status", "arc_sdpa_launch_count",
     "arc_plan_head_shards", "arc_plan_seq_shards", "arc_plan_batch_shards", "arc_sdpa_exchange_init", "arc_sdpa_record_floats",
     "arc_sdpa_allgather_merge",
+    "arc_paged_tables", "arc_qkv_prepare_paged", "arc_sdpa_decode_paged_workspace_bytes", "arc_sdpa_decode_paged",
 )
 
 
@@ -56,7 +57,7 @@ class PrefillParams(C.Structure):
         ("scale", C.c_float), ("mask_type", C.c_int32), ("window", C.c_int32), ("num_splits", C.c_int32),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("block_ids", C.c_void_p), ("block_ids_offset", C.c_int32),
-        ("out_copies", C.c_void_p), ("out_copy_count", C.c_int32),
+        ("out_copies", C.c_void_p), ("out_copy_count", C.c_int32), ("sinks", C.c_int32),
     ]
 
 
@@ -95,6 +96,45 @@ class QkvPrepareParams(C.Structure):
         ("pos0", C.c_int32), ("theta", C.c_float), ("eps", C.c_float),
         ("rot_half", C.c_int32), ("freq_denom", C.c_int32), ("mrope_positions", C.c_void_p),
         ("mrope_section", C.c_int32 * 3), ("v_copy", C.c_int32),
+    ]
+
+
+class PagedTablesParams(C.Structure):
+    _fields_ = [
+        ("new_len", C.c_void_p), ("past_len", C.c_void_p), ("block_table", C.c_void_p), ("free_pages", C.c_void_p),
+        ("free_begin", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p), ("token_begin", C.c_void_p),
+        ("kv_len", C.c_void_p), ("pages_used", C.c_void_p),
+        ("batch", C.c_int32), ("num_tokens", C.c_int32), ("page_size", C.c_int32), ("table_width", C.c_int32), ("free_count", C.c_int32),
+        ("table_stride", C.c_int64),
+    ]
+
+
+class QkvPreparePagedParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p), ("inv_freq", C.c_void_p),
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+        ("tokens", C.c_int32), ("nq", C.c_int32), ("nkv", C.c_int32), ("hd", C.c_int32),
+        ("page_size", C.c_int32), ("num_pages", C.c_int32),
+        ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("norm_qk", C.c_int32), ("norm_v", C.c_int32),
+        ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64),
+        ("k_out_stride", C.c_int64), ("v_out_stride", C.c_int64),
+        ("k_stride_page", C.c_int64), ("k_stride_t", C.c_int64), ("v_stride_page", C.c_int64), ("v_stride_t", C.c_int64),
+        ("eps", C.c_float), ("mscale", C.c_float),
+    ]
+
+
+class DecodePagedParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("out", C.c_void_p), ("gate", C.c_void_p),
+        ("block_table", C.c_void_p), ("kv_len", C.c_void_p), ("out_f32", C.c_void_p), ("out_lse", C.c_void_p),
+        ("batch", C.c_int32), ("nq", C.c_int32), ("nkv", C.c_int32), ("hd", C.c_int32),
+        ("page_size", C.c_int32), ("num_pages", C.c_int32), ("table_width", C.c_int32), ("kv_len_uniform", C.c_int32),
+        ("window", C.c_int32), ("sinks", C.c_int32),
+        ("q_stride_b", C.c_int64), ("o_stride_b", C.c_int64), ("table_stride", C.c_int64),
+        ("k_stride_page", C.c_int64), ("k_stride_t", C.c_int64), ("v_stride_page", C.c_int64), ("v_stride_t", C.c_int64),
+        ("scale", C.c_float), ("num_ctas", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -156,6 +196,14 @@ def load() -> C.CDLL:
     L.arc_sdpa_record_floats.argtypes = [C.c_int32, C.c_int32, C.c_int32]
     L.arc_sdpa_allgather_merge.restype = C.c_int
     L.arc_sdpa_allgather_merge.argtypes = [vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, vp, vp, vp, vp]
+    L.arc_paged_tables.restype = C.c_int
+    L.arc_paged_tables.argtypes = [C.POINTER(PagedTablesParams), vp]
+    L.arc_qkv_prepare_paged.restype = C.c_int
+    L.arc_qkv_prepare_paged.argtypes = [C.POINTER(QkvPreparePagedParams), vp]
+    L.arc_sdpa_decode_paged_workspace_bytes.restype = C.c_size_t
+    L.arc_sdpa_decode_paged_workspace_bytes.argtypes = [C.POINTER(DecodePagedParams)]
+    L.arc_sdpa_decode_paged.restype = C.c_int
+    L.arc_sdpa_decode_paged.argtypes = [C.POINTER(DecodePagedParams), vp]
     _lib = L
     return L
 

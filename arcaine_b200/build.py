@@ -8,6 +8,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -44,12 +45,14 @@ def sources() -> list[str]:
 def build_library(force: bool = False, verbose: bool = False) -> str:
     """Compile every kernel and the C ABI into ``libarc_sdpa.so``."""
     if force or _stale(LIB, sources()):
-        cmd = [_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB,
-               os.path.join(CSRC, "arc_sdpa.cu"), os.path.join(CSRC, "arcaine_attention.cpp"),
-               os.path.join(CSRC, "arc_multi_gpu.cpp"), "-ldl"]
-        if verbose:
-            cmd.insert(1, "-Xptxas=-v")
-        subprocess.check_call(cmd)
+        units = ("arc_sdpa.cu", "arc_paged.cu", "arcaine_attention.cpp", "arc_multi_gpu.cpp")
+        with tempfile.TemporaryDirectory() as tmp:  # side by side: the kernels of one file take a minute
+            objects = [os.path.join(tmp, u + ".o") for u in units]
+            jobs = [subprocess.Popen([_nvcc(), *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS, "-c", os.path.join(CSRC, u), "-o", o])
+                    for u, o in zip(units, objects)]
+            if any([job.wait() != 0 for job in jobs]):
+                raise RuntimeError("nvcc failed")
+            subprocess.check_call([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB, *objects, "-ldl"])
     return LIB
 
 

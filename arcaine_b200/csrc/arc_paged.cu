@@ -1,0 +1,297 @@
+// C ABI of the paged KV cache: tables, pre-processing with append, decode.  Argument checks, launch plans, launches.
+#include "../../include/arc_sdpa.h"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "arc_internal.hpp"
+#include "decode_paged_sm100.cuh"
+#include "paged_sm100.cuh"
+
+using namespace arc;
+
+// Strides of a pool of pages: rows must hold a token's heads, pages their rows.
+static int check_pool(int64_t stride_page, int64_t stride_t, int page_size, int num_pages, int64_t row) {
+    if (stride_page < 0 || stride_t < 0 || (stride_page & 7) || (stride_t & 7)) return ARC_ERR_ALIGNMENT;
+    if (stride_t < row || (num_pages > 1 && stride_page < (page_size - 1) * stride_t + row)) return ARC_ERR_BAD_SHAPE;
+    return ARC_OK;
+}
+
+static int check_pages(int page_size, int num_pages) {
+    if (page_size < 16 || page_size % 16 != 0 || num_pages < 1) return ARC_ERR_BAD_SHAPE;
+    if ((int64_t)page_size * num_pages > 0x7fffffffLL) return ARC_ERR_TOO_LARGE;  // (slots are 32 bits wide)
+    return ARC_OK;
+}
+
+extern "C" int arc_paged_tables(const arc_paged_tables_params* p, void* stream) {
+    if (!p) return ARC_ERR_NULL_POINTER;
+    if (p->batch <= 0 || p->num_tokens < 0 || p->table_width < 1 || p->free_count < 0 || p->table_stride < p->table_width ||
+        p->page_size < 16 || p->page_size % 16 != 0)
+        return ARC_ERR_BAD_SHAPE;
+    if (p->batch > TABLES_MAX_BATCH) return ARC_ERR_TOO_LARGE;
+    if (!p->new_len || !p->block_table || (p->free_count > 0 && !p->free_pages) || (p->num_tokens > 0 && (!p->slots || !p->positions)) ||
+        !p->token_begin || !p->kv_len || !p->pages_used)
+        return ARC_ERR_NULL_POINTER;
+    const void* all[] = {p->new_len, p->past_len, p->block_table, p->free_pages, p->free_begin, p->slots, p->positions, p->token_begin, p->kv_len, p->pages_used};
+    for (const void* a : all)
+        if (reinterpret_cast<uintptr_t>(a) & 3u) return ARC_ERR_ALIGNMENT;
+    HostState hs;
+    const int rc = host_state(&hs);
+    if (rc != ARC_OK) return rc;
+    PagedTablesParams kp{};
+    kp.new_len = p->new_len;
+    kp.past_len = p->past_len;
+    kp.table = p->block_table;
+    kp.free_pages = p->free_pages;
+    kp.free_begin = p->free_begin;
+    kp.slots = p->slots;
+    kp.positions = p->positions;
+    kp.token_begin = p->token_begin;
+    kp.kv_len = p->kv_len;
+    kp.pages_used = p->pages_used;
+    kp.fault = hs.fault;
+    kp.batch = p->batch;
+    kp.num_tokens = p->num_tokens;
+    kp.page = p->page_size;
+    kp.width = p->table_width;
+    kp.free_count = p->free_count;
+    kp.table_stride = p->table_stride;
+    const int blocks = std::max(1, std::min(hs.sm_count * 2, (p->num_tokens + TABLES_THREADS - 1) / TABLES_THREADS));
+    ARC_CUDA(launch_dependent(paged_tables_kernel, dim3((unsigned)blocks), dim3(TABLES_THREADS), 0, static_cast<cudaStream_t>(stream), 1, kp));
+    count_launch();
+    return ARC_OK;
+}
+
+extern "C" int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void* stream) {
+    if (!p) return ARC_ERR_NULL_POINTER;
+    if (p->hd != 128 && p->hd != 256 && p->hd != 512) return ARC_ERR_UNSUPPORTED_HEAD_DIM;
+    if (p->tokens < 0 || (p->q && p->nq < 1) || (p->k && p->nkv < 1)) return ARC_ERR_BAD_SHAPE;
+    if (p->rotary_dim < 0 || p->rotary_dim > p->hd || p->rotary_dim % 16 != 0) return ARC_ERR_BAD_SHAPE;
+    if (!std::isfinite(p->eps) || p->eps < 0.f || !std::isfinite(p->mscale)) return ARC_ERR_BAD_SHAPE;
+    if (p->v && !p->k) return ARC_ERR_NULL_POINTER;
+    if ((p->q && !p->q_out) || (p->k && !p->k_out && !p->k_pages) || (p->v && !p->v_out && !p->v_pages)) return ARC_ERR_NULL_POINTER;
+    if ((p->rotary_dim > 0 && !p->inv_freq) || !p->positions) return ARC_ERR_NULL_POINTER;
+    const bool pages = (p->k && p->k_pages) || (p->v && p->v_pages);
+    if (pages && !p->slots) return ARC_ERR_NULL_POINTER;
+    if (!p->q && !p->k) return ARC_ERR_NULL_POINTER;
+    const void* all[] = {p->q, p->k, p->v, p->q_out, p->k_out, p->v_out, p->k_pages, p->v_pages, p->q_weight, p->k_weight};
+    for (const void* a : all)
+        if (!aligned16(a)) return ARC_ERR_ALIGNMENT;
+    if ((reinterpret_cast<uintptr_t>(p->inv_freq) & 7u) || (reinterpret_cast<uintptr_t>(p->slots) & 3u) || (reinterpret_cast<uintptr_t>(p->positions) & 3u))
+        return ARC_ERR_ALIGNMENT;
+    const int64_t qrow = (int64_t)p->nq * p->hd, row = (int64_t)p->nkv * p->hd;
+    int rc;
+    const auto tokens_apart = [](bool used, int64_t stride, int64_t least) {
+        if (!used) return ARC_OK;
+        if (stride < 0 || (stride & 7)) return ARC_ERR_ALIGNMENT;
+        return stride < least ? ARC_ERR_BAD_SHAPE : ARC_OK;
+    };
+    if ((rc = tokens_apart(p->q, p->q_stride, qrow)) != ARC_OK || (rc = tokens_apart(p->q, p->q_out_stride, qrow)) != ARC_OK ||
+        (rc = tokens_apart(p->k, p->k_stride, row)) != ARC_OK || (rc = tokens_apart(p->v, p->v_stride, row)) != ARC_OK ||
+        (rc = tokens_apart(p->k && p->k_out, p->k_out_stride, row)) != ARC_OK || (rc = tokens_apart(p->v && p->v_out, p->v_out_stride, row)) != ARC_OK)
+        return rc;
+    if (pages) {
+        if ((rc = check_pages(p->page_size, p->num_pages)) != ARC_OK) return rc;
+        if (p->k_pages && (rc = check_pool(p->k_stride_page, p->k_stride_t, p->page_size, p->num_pages, row)) != ARC_OK) return rc;
+        if (p->v && p->v_pages && (rc = check_pool(p->v_stride_page, p->v_stride_t, p->page_size, p->num_pages, row)) != ARC_OK) return rc;
+    }
+    if (p->tokens == 0) return ARC_OK;
+    HostState hs;
+    if ((rc = host_state(&hs)) != ARC_OK) return rc;
+
+    QkvPagedParams kp{};
+    const void* src[3] = {p->q, p->k, p->v};
+    void* out[3] = {p->q_out, p->k_out, p->v_out};
+    void* pool[3] = {nullptr, p->k_pages, p->v_pages};
+    const int64_t src_stride[3] = {p->q_stride, p->k_stride, p->v_stride}, out_stride[3] = {p->q_out_stride, p->k_out_stride, p->v_out_stride};
+    const int64_t page_stride[3] = {0, p->k_stride_page, p->v_stride_page}, row_stride[3] = {0, p->k_stride_t, p->v_stride_t};
+    int rows = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (src[i]) {
+            kp.src[i] = static_cast<const uint16_t*>(src[i]);
+            kp.out[i] = static_cast<uint16_t*>(out[i]);
+            kp.pages[i] = static_cast<uint16_t*>(pool[i]);
+            kp.src_stride[i] = src_stride[i];
+            kp.out_stride[i] = out_stride[i];
+            kp.page_stride[i] = page_stride[i];
+            kp.row_stride[i] = row_stride[i];
+            rows += i == 0 ? p->nq : p->nkv;
+        }
+        kp.end[i] = rows;
+    }
+    kp.slots = pages ? p->slots : nullptr;
+    kp.positions = p->positions;
+    kp.inv_freq = p->inv_freq;
+    kp.weight[0] = static_cast<const uint16_t*>(p->q_weight);
+    kp.weight[1] = static_cast<const uint16_t*>(p->k_weight);
+    kp.fault = hs.fault;
+    kp.tokens = p->tokens;
+    kp.page = pages ? p->page_size : 1;
+    kp.num_rows = pages ? p->page_size * p->num_pages : 0;
+    kp.half = p->rotary_dim / 2;
+    kp.norm_qk = p->norm_qk != 0;
+    kp.norm_v = p->norm_v != 0;
+    kp.eps = p->eps;
+    kp.mscale = p->mscale;
+    // A warp takes a token at a time, or a part of a token's passes: whatever gives the last warp the fewest passes, the start of
+    // a unit (the token's angles) counted as one; whole tokens where there are several for every warp.
+    const int passes = (rows + 512 / p->hd - 1) / (512 / p->hd);
+    const long long warps = (long long)hs.sm_count * 2 * PREP_WARPS;
+    int chunk = passes, chunks = 1;
+    long long best = 0;
+    for (int c = passes; p->tokens < 4 * warps; c = (c + 1) / 2) {
+        const int n = (passes + c - 1) / c;
+        const long long cost = ((long long)p->tokens * n + warps - 1) / warps * (c + 1);
+        if (best == 0 || cost < best) best = cost, chunk = c, chunks = n;
+        if (c == 1) break;
+    }
+    if ((long long)p->tokens * chunks + warps > 0x7fffffffLL) return ARC_ERR_TOO_LARGE;
+    const long long units = (long long)p->tokens * chunks;
+    const unsigned ctas = (unsigned)((std::min(units, warps) + PREP_WARPS - 1) / PREP_WARPS);
+    auto launch = [&](auto hd_tag) {
+        constexpr int H = decltype(hd_tag)::value;
+        return launch_dependent(p->interleaved ? qkv_prepare_paged_kernel<H, true> : qkv_prepare_paged_kernel<H, false>, dim3(ctas), dim3(32 * PREP_WARPS), 0,
+                                static_cast<cudaStream_t>(stream), 1, kp, chunk, chunks);
+    };
+    ARC_CUDA(p->hd == 128 ? launch(std::integral_constant<int, 128>{}) : p->hd == 256 ? launch(std::integral_constant<int, 256>{}) : launch(std::integral_constant<int, 512>{}));
+    count_launch();
+    return ARC_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Decode
+// ---------------------------------------------------------------------------
+struct DecodePagedPlan {
+    int nkv_cta = 1, groups = 1, slices = 1, stages = 2, ncta = 1, nt = 1, smem_bytes = 0;
+    long long parts = 0;
+    size_t ws_bytes = 0;
+};
+
+static int plan_decode_paged(const arc_sdpa_decode_paged_params* p, const HostState& hs, DecodePagedPlan* plan) {
+    if (!p) return ARC_ERR_NULL_POINTER;
+    if (p->batch <= 0 || p->nq <= 0 || p->nkv <= 0 || p->nq % p->nkv != 0 || p->table_width < 1 || p->table_stride < p->table_width)
+        return ARC_ERR_BAD_SHAPE;
+    if (p->batch > DECODE_MAX_BATCH) return ARC_ERR_TOO_LARGE;
+    if (p->hd != 128 && p->hd != 256) return ARC_ERR_UNSUPPORTED_HEAD_DIM;
+    if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return ARC_ERR_BAD_SHAPE;
+    if (p->window < 1 || p->sinks < 0 || p->num_ctas < 0) return ARC_ERR_BAD_SHAPE;
+    int rc = check_pages(p->page_size, p->num_pages);
+    if (rc != ARC_OK) return rc;
+    if (!p->kv_len && (p->kv_len_uniform < 0 || p->kv_len_uniform > (int64_t)p->table_width * p->page_size)) return ARC_ERR_BAD_SHAPE;
+    const int G = p->nq / p->nkv;
+    if (G > 16) return ARC_ERR_UNSUPPORTED_GQA;
+    plan->nt = G > 8 ? 2 : 1;
+    // KV heads of a CTA: the largest divisor of nkv whose rows are at most 2 KB; slices of a stage: 64 KB of K and V, eight warps.
+    for (int c = 1; c <= p->nkv && c <= 1024 / p->hd; ++c)
+        if (p->nkv % c == 0) plan->nkv_cta = c;
+    plan->slices = std::max(1, std::min(64 * 1024 / (64 * plan->nkv_cta * p->hd), 8 / plan->nkv_cta));
+    const int stage = 64 * plan->slices * plan->nkv_cta * p->hd, fixed = 1024 + 4 * 16 + (p->batch + 2) * 8;
+    plan->stages = std::min(4, (hs.smem_optin - kDecodeStaticSmem - fixed) / stage);
+    if (plan->stages < 2) return ARC_ERR_TOO_LARGE;
+    plan->smem_bytes = plan->stages * stage + fixed;
+    plan->groups = p->nkv / plan->nkv_cta;
+    plan->ncta = std::min(1024, std::max(1, p->num_ctas > 0 ? p->num_ctas : hs.sm_count / plan->groups));
+    plan->parts = ((long long)plan->ncta + p->batch) * plan->slices;
+    plan->ws_bytes = (size_t)plan->parts * p->nq * ((size_t)p->hd + 1) * sizeof(float);
+    return ARC_OK;
+}
+
+// A pool of pages as (64 columns, row, 64-column chunk, KV head, page); box: 16 rows of `heads` heads.
+static int make_pool_map(CUtensorMap* tm, const void* base, int hd, int nkv, int heads, int page, int num_pages, int64_t stride_t, int64_t stride_page) {
+    const cuuint64_t dims[5] = {64u, (cuuint64_t)page, (cuuint64_t)hd / 64u, (cuuint64_t)nkv, (cuuint64_t)num_pages};
+    const cuuint64_t last = (cuuint64_t)(num_pages > 1 ? stride_page : stride_t * page);
+    const cuuint64_t strides[4] = {(cuuint64_t)stride_t * 2u, 128u, (cuuint64_t)hd * 2u, last * 2u};
+    const cuuint32_t box[5] = {64u, 16u, (cuuint32_t)hd / 64u, (cuuint32_t)heads, 1u};
+    return encode_bf16_map(tm, base, 5, dims, strides, box, " (pages)");
+}
+
+template <int HD>
+static int launch_decode_paged(const arc_sdpa_decode_paged_params* p, const DecodePagedPlan& plan, const HostState& hs, cudaStream_t stream) {
+    CUtensorMap tk, tv;
+    int rc;
+    if ((rc = make_pool_map(&tk, p->k_pages, HD, p->nkv, plan.nkv_cta, p->page_size, p->num_pages, p->k_stride_t, p->k_stride_page)) != ARC_OK) return rc;
+    if ((rc = make_pool_map(&tv, p->v_pages, HD, p->nkv, plan.nkv_cta, p->page_size, p->num_pages, p->v_stride_t, p->v_stride_page)) != ARC_OK) return rc;
+    DecodePagedParams kp{};
+    kp.q = static_cast<const uint16_t*>(p->q);
+    kp.table = p->block_table;
+    kp.kv_len = p->kv_len;
+    kp.part_o = static_cast<float*>(p->workspace);
+    kp.part_lse = kp.part_o + (size_t)plan.parts * p->nq * HD;
+    kp.fault = hs.fault;
+    kp.batch = p->batch;
+    kp.nq = p->nq;
+    kp.nkv = p->nkv;
+    kp.kv_len_uniform = p->kv_len_uniform;
+    kp.page = p->page_size;
+    kp.num_pages = p->num_pages;
+    kp.max_len = (int)std::min<int64_t>((int64_t)p->table_width * p->page_size, 0x7fffffffLL - 16);
+    kp.window = p->window;
+    kp.sinks = p->sinks;
+    kp.q_stride_b = p->q_stride_b;
+    kp.table_stride = p->table_stride;
+    kp.scale_log2 = p->scale * 1.4426950408889634f;
+    kp.nkv_cta = plan.nkv_cta;
+    kp.slices = plan.slices;
+    kp.stages = plan.stages;
+    kp.ncta = plan.ncta;
+    const auto kernel = plan.nt == 1 ? sdpa_decode_paged_kernel<HD, 1> : sdpa_decode_paged_kernel<HD, 2>;
+    ARC_CUDA(opt_in_smem(kernel, hs.smem_optin - kDecodeStaticSmem));
+    ARC_CUDA(launch_dependent(kernel, dim3((unsigned)plan.ncta, (unsigned)plan.groups), dim3(32u * (unsigned)(plan.nkv_cta * plan.slices + 1)),
+                              (size_t)plan.smem_bytes, stream, 1, tk, tv, kp));
+    count_launch();
+
+    DecodeMergeParams mp{};
+    mp.part_o = kp.part_o;
+    mp.part_lse = kp.part_lse;
+    mp.kv_len = p->kv_len;
+    mp.gate = static_cast<const uint16_t*>(p->gate);
+    mp.out = static_cast<uint16_t*>(p->out);
+    mp.out_f32 = p->out_f32;
+    mp.out_lse = p->out_lse;
+    mp.batch = p->batch;
+    mp.nq = p->nq;
+    mp.kv_len_uniform = p->kv_len_uniform;
+    mp.ncta = plan.ncta;
+    mp.slices = plan.slices;
+    mp.o_stride_b = p->o_stride_b;
+    mp.fault = hs.fault;
+    mp.window = p->window;
+    mp.sinks = p->sinks;
+    // 64 columns a block while that leaves at most one block per SM (arc_sdpa.cu).
+    const bool narrow = (long long)p->nq * p->batch * (HD / 64) <= hs.sm_count;
+    ARC_CUDA(launch_dependent(narrow ? sdpa_decode_merge_kernel<HD, false, 64, true> : sdpa_decode_merge_kernel<HD, false, HD, true>,
+                              dim3((unsigned)p->nq, (unsigned)p->batch, narrow ? HD / 64 : 1), dim3(MERGE_THREADS), 0, stream, 1, mp));
+    count_launch();
+    return ARC_OK;
+}
+
+extern "C" size_t arc_sdpa_decode_paged_workspace_bytes(const arc_sdpa_decode_paged_params* p) {
+    HostState hs;
+    DecodePagedPlan plan;
+    if (host_state(&hs) != ARC_OK || plan_decode_paged(p, hs, &plan) != ARC_OK) return 0;
+    return plan.ws_bytes;
+}
+
+extern "C" int arc_sdpa_decode_paged(const arc_sdpa_decode_paged_params* p, void* stream) {
+    if (!p || !p->q || !p->k_pages || !p->v_pages || !p->block_table || (!p->out && !p->out_f32) || (p->gate && !p->out)) return ARC_ERR_NULL_POINTER;
+    // What needs no device is refused without one.
+    DecodePagedPlan plan;
+    int rc = plan_decode_paged(p, HostState{nullptr, 148, 232448}, &plan);
+    if (rc != ARC_OK) return rc;
+    if (!aligned16(p->q) || !aligned16(p->k_pages) || !aligned16(p->v_pages) || !aligned16(p->out) || !aligned16(p->gate) || !aligned16(p->out_f32) ||
+        ((reinterpret_cast<uintptr_t>(p->block_table) | reinterpret_cast<uintptr_t>(p->kv_len) | reinterpret_cast<uintptr_t>(p->out_lse)) & 3u) ||
+        (p->q_stride_b & 7) || (p->o_stride_b & 7))
+        return ARC_ERR_ALIGNMENT;
+    const int64_t qrow = (int64_t)p->nq * p->hd;
+    if (p->batch > 1 && (p->q_stride_b < qrow || (p->out && p->o_stride_b < qrow))) return ARC_ERR_BAD_SHAPE;
+    if ((rc = check_pool(p->k_stride_page, p->k_stride_t, p->page_size, p->num_pages, (int64_t)p->nkv * p->hd)) != ARC_OK ||
+        (rc = check_pool(p->v_stride_page, p->v_stride_t, p->page_size, p->num_pages, (int64_t)p->nkv * p->hd)) != ARC_OK)
+        return rc;
+    HostState hs;
+    if ((rc = host_state(&hs)) != ARC_OK || (rc = plan_decode_paged(p, hs, &plan)) != ARC_OK) return rc;
+    if (!p->workspace || p->workspace_bytes < plan.ws_bytes) return ARC_ERR_WORKSPACE_TOO_SMALL;
+    if (!aligned16(p->workspace)) return ARC_ERR_ALIGNMENT;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return p->hd == 128 ? launch_decode_paged<128>(p, plan, hs, st) : launch_decode_paged<256>(p, plan, hs, st);
+}

@@ -16,6 +16,7 @@
 #include <type_traits>
 #include <mutex>
 
+#include "arc_internal.hpp"
 #include "decode_sm100.cuh"
 #include "prefill_pair_sm100.cuh"
 #include "qkv_prepare_sm100.cuh"
@@ -29,9 +30,6 @@ namespace arc {
 __device__ uint32_t g_fault_words[2];
 
 constexpr int kMaxDevices = 64;
-// The decode kernel keeps a few bytes of static shared memory; the dynamic part
-// may use the opt-in maximum minus this reserve.
-constexpr int kDecodeStaticSmem = 1024;
 
 // What the device holds of the CTA pairs of prefill_wide_sm100.cuh at once (the defaults: a B200).
 struct WideRoom {
@@ -62,21 +60,10 @@ static EncodeTiledFn g_encode = nullptr;
 // Text of the most recent failing CUDA call on this thread (for diagnostics).
 static thread_local char g_last_error[256] = "";
 
-static int cuda_fail(const char* what, cudaError_t e) {
+int cuda_fail(const char* what, cudaError_t e) {
     std::snprintf(g_last_error, sizeof(g_last_error), "%s: %s", what, cudaGetErrorString(e));
     cudaGetLastError();
     return ARC_ERR_CUDA;
-}
-
-#define ARC_CUDA(call)                                      \
-    do {                                                    \
-        cudaError_t e_ = (call);                            \
-        if (e_ != cudaSuccess) return cuda_fail(#call, e_); \
-    } while (0)
-
-template <typename K>
-static cudaError_t opt_in_smem(K kernel, int bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 // How many clusters of `size` CTAs of a kernel the device holds at once (0: none).
@@ -103,20 +90,28 @@ static int clusters_at_once(K kernel, int size, int sm_count, int threads, int s
 
 // The instances of the kernels of head dim 128 for a call; the common ones carry nothing they do not need.
 using PairKernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PrefillParams);
-static PairKernel pair_kernel(bool gate, bool copies, bool vision) {
+static PairKernel pair_kernel(bool gate, bool copies, bool vision, bool sinks = false) {
+    if (sinks) return gate ? sdpa_prefill_pair_kernel<true, true, false, true> : copies ? sdpa_prefill_pair_kernel<false, true, false, true> : sdpa_prefill_pair_kernel<false, false, false, true>;
     if (vision) return gate ? sdpa_prefill_pair_kernel<true, true, true> : copies ? sdpa_prefill_pair_kernel<false, true, true> : sdpa_prefill_pair_kernel<false, false, true>;
     if (copies) return gate ? sdpa_prefill_pair_kernel<true, true> : sdpa_prefill_pair_kernel<false, true>;
     return gate ? sdpa_prefill_pair_kernel<true, false> : sdpa_prefill_pair_kernel<false, false>;
 }
 using ChainsKernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, PrefillParams);
-static ChainsKernel chains_kernel(bool gate, bool vision, bool masked) {
+static ChainsKernel chains_kernel(bool gate, bool vision, bool masked, bool sinks = false) {
+    if (sinks) return gate ? sdpa_prefill_chains_kernel<true, false, false, true> : sdpa_prefill_chains_kernel<false, false, false, true>;
     if (masked) return gate ? sdpa_prefill_chains_kernel<true, false, true> : sdpa_prefill_chains_kernel<false, false, true>;
     if (vision) return gate ? sdpa_prefill_chains_kernel<true, true, false> : sdpa_prefill_chains_kernel<false, true, false>;
     return gate ? sdpa_prefill_chains_kernel<true, false, false> : sdpa_prefill_chains_kernel<false, false, false>;
 }
 
 using WideKernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PrefillParams);
-static WideKernel wide_kernel(bool gate, bool masked, int split, bool several, bool vision) {  // (several: units per CTA pair)
+static WideKernel wide_kernel(bool gate, bool masked, int split, bool several, bool vision, bool sinks = false) {  // (several: units per CTA pair)
+    if (sinks) {
+        if (split == 2) return gate ? sdpa_prefill_wide_kernel<true, false, 2, false, false, true> : sdpa_prefill_wide_kernel<false, false, 2, false, false, true>;
+        if (split == 1) return sdpa_prefill_wide_kernel<false, false, 1, false, false, true>;
+        if (several) return gate ? sdpa_prefill_wide_kernel<true, false, 0, true, false, true> : sdpa_prefill_wide_kernel<false, false, 0, true, false, true>;
+        return gate ? sdpa_prefill_wide_kernel<true, false, 0, false, false, true> : sdpa_prefill_wide_kernel<false, false, 0, false, false, true>;
+    }
     if (split == 2 && gate) return masked ? sdpa_prefill_wide_kernel<true, true, 2> : vision ? sdpa_prefill_wide_kernel<true, false, 2, false, true> : sdpa_prefill_wide_kernel<true, false, 2>;
     if (split == 2) return masked ? sdpa_prefill_wide_kernel<false, true, 2> : vision ? sdpa_prefill_wide_kernel<false, false, 2, false, true> : sdpa_prefill_wide_kernel<false, false, 2>;
     if (split == 1) return masked ? sdpa_prefill_wide_kernel<false, true, 1> : vision ? sdpa_prefill_wide_kernel<false, false, 1, false, true> : sdpa_prefill_wide_kernel<false, false, 1>;
@@ -154,12 +149,12 @@ static int device_state(DeviceState** out) {
                 }
                 g_encode = reinterpret_cast<EncodeTiledFn>(fn);
             }
-            for (int i = 0; i < 8; ++i) {
-                ARC_CUDA(opt_in_smem(pair_kernel(i & 1, i & 2, i & 4), PairCfg::SMEM_BYTES));
-                ARC_CUDA(opt_in_smem(chains_kernel(i & 1, i & 2, i & 4), ChainsCfg::SMEM_BYTES));
+            for (int i = 0; i < 16; ++i) {
+                ARC_CUDA(opt_in_smem(pair_kernel(i & 1, i & 2, i & 4, i & 8), PairCfg::SMEM_BYTES));
+                ARC_CUDA(opt_in_smem(chains_kernel(i & 1, i & 2, i & 4, i & 8), ChainsCfg::SMEM_BYTES));
             }
             ARC_CUDA(opt_in_smem(sdpa_prefill_kernel, PrefillCfg::SMEM_BYTES));
-            for (int i = 0; i < 48; ++i) ARC_CUDA(opt_in_smem(wide_kernel(i & 1, i & 2, i / 16, i & 4, i & 8), WideCfg::SMEM_BYTES));
+            for (int i = 0; i < 96; ++i) ARC_CUDA(opt_in_smem(wide_kernel(i & 1, i & 2, i / 16 % 3, i & 4, i & 8, i >= 48), WideCfg::SMEM_BYTES));
             s.wide.pairs = clusters_at_once(sdpa_prefill_wide_kernel<false, false>, 2, s.sm_count, WideCfg::THREADS, WideCfg::SMEM_BYTES);
             for (int parts = 2; parts <= WideRoom::MOST_FOLDED; ++parts)
                 s.wide.folded[parts] = clusters_at_once(sdpa_prefill_wide_kernel<false, false, 2>, 2 * parts, s.sm_count, WideCfg::THREADS, WideCfg::SMEM_BYTES);
@@ -188,33 +183,25 @@ static int device_state(DeviceState** out) {
     return ARC_OK;
 }
 
-// Launch `kernel` behind the previous kernel of `stream` with programmatic serialization: its CTAs may be scheduled and
-// run up to their grid_dependency_wait() while that kernel is still running, which takes the launch latency and the
-// prologue off the critical path (2-3 us of a small call).  Every kernel of the library is launched this way, and every
-// one of them waits before it touches global memory and only then releases the kernel behind it
-// (grid_launch_dependents): so when a kernel may run, everything in front of its predecessor has completed, and no grid
-// completes before the one in front of it has.  cluster > 1: in clusters of that many CTAs along x.
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster,
-                                    Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+int host_state(HostState* out) {
+    DeviceState* ds = nullptr;
+    const int rc = device_state(&ds);
+    if (rc == ARC_OK) *out = HostState{ds->fault, ds->sm_count, ds->smem_optin};
+    return rc;
 }
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
+int encode_bf16_map(CUtensorMap* tm, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                    const char* what) {
+    const cuuint32_t estr[5] = {1u, 1u, 1u, 1u, 1u};
+    const CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return ARC_OK;
+    std::snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled%s failed with CUresult %d", what, (int)r);
+    return ARC_ERR_CUDA;
+}
 
 // (hd, heads, tokens, batch) view of a token-major bf16 tensor; box = 64 x 1 x box_rows x 1, 128-byte swizzle.
 static int make_tile_map(CUtensorMap* tm, const void* base, int hd, int heads, int tokens, int batch,
@@ -223,15 +210,7 @@ static int make_tile_map(CUtensorMap* tm, const void* base, int hd, int heads, i
     cuuint64_t sb = (cuuint64_t)(batch > 1 ? stride_b : stride_t * (int64_t)tokens) * 2u;
     cuuint64_t strides[3] = {(cuuint64_t)hd * 2u, (cuuint64_t)stride_t * 2u, sb};
     cuuint32_t box[4] = {64u, 1u, (cuuint32_t)box_rows, 1u};
-    cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-    CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        std::snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-        return ARC_ERR_CUDA;
-    }
-    return ARC_OK;
+    return encode_bf16_map(tm, base, 4, dims, strides, box, "");
 }
 
 // Output and gate as the epilogue warps see them: boxes of 64 columns x 32 rows.
@@ -251,15 +230,7 @@ static int make_cache_map(CUtensorMap* tm, const void* base, int row_elems, int6
     cuuint64_t dims[2] = {(cuuint64_t)row_elems, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)stride_t * 2u};
     cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
-    cuuint32_t estr[2] = {1u, 1u};
-    CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        std::snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled (cache) failed with CUresult %d", (int)r);
-        return ARC_ERR_CUDA;
-    }
-    return ARC_OK;
+    return encode_bf16_map(tm, base, 2, dims, strides, box, " (cache)");
 }
 
 // ---------------------------------------------------------------------------
@@ -273,13 +244,16 @@ struct PrefillPlan {
     size_t mask_bytes = 0;  // behind it, if it is there: the classes and bits of an additive mask
 };
 
+// Keys that stay visible behind a call's window.  (Without a window, or behind one that hides nothing, there is nothing to keep visible.)
+static int sinks_of(const arc_sdpa_prefill_params* p) { return p->window > 0 && p->window < p->kv_len ? p->sinks : 0; }
+
 // Key blocks that token tile qt (128 rows) of a call sees, block ids apart.
 static int tile_key_blocks(const arc_sdpa_prefill_params* p, int qt) {
     const int blocks = (p->kv_len + 127) / 128, off = p->kv_len - p->seq;
     if (p->mask_type != ARC_MASK_CAUSAL) return blocks;
     const int last = std::min(p->kv_len - 1, std::min(qt * 128 + 127, p->seq - 1) + off);
     const int hi = last >= 0 ? last / 128 + 1 : 0, lo = p->window > 0 && p->window != 0x7fffffff ? std::max(0, qt * 128 + off - p->window + 1) / 128 : 0;
-    return std::max(0, hi - lo);
+    return std::max(0, hi - lo) + std::min((sinks_of(p) + 127) / 128, lo);
 }
 
 // Head dim 256: units of the CTA pairs' list.
@@ -326,7 +300,7 @@ static int choose_wide_splits(const arc_sdpa_prefill_params* p, int q_tiles, con
     // bias per key, 128 queries of 16 heads over 4096 keys: 116 us whole).
     if (masked && most <= 24 && (long long)p->batch * p->seq * p->nq > 1024) return 1;
     if (windowed) {
-        most = std::min(most, (p->window + 255) / 128 + 1);
+        most = std::min(most, (p->window + 255) / 128 + 1 + (sinks_of(p) + 127) / 128);
         // (That is the most that a window can cover, up to two more than it does.  Gated calls, whose epilogue and merge weigh more, are
         // divided by what it does: 256 queries of 8 heads over 1500 keys, window 533, 11.5 us in three parts, 13.2 in four.  For the others
         // the bound is the better guess: 63 of 24 heads over 1000 keys 9.9 in four, 10.4 in three.)
@@ -381,10 +355,11 @@ static int plan_prefill(const arc_sdpa_prefill_params* p, int sm_count, const Wi
         // (8 tiles of 12 / 16 / 32 blocks: 12.4 / 16.1 / 28.9 us whole, 10.6 / 11.3 / 14.5 in four parts, 10.5 / 10.7 / 12.3 in
         // eight; 32 tiles of 16: 16.8 whole, 16.2 in two, 13.5 in four.)
         splits = 1;
-        if (tiles * 2 <= sm_count && kv_blocks >= 10) {
+        const int seen = sinks_of(p) ? std::min(kv_blocks, (p->window + 255) / 128 + 1 + (sinks_of(p) + 127) / 128) : kv_blocks;
+        if (tiles * 2 <= sm_count && seen >= 10) {
             double least = 1e30;
-            for (int s = 2; s <= 8 && 2 * s <= kv_blocks && tiles * s <= sm_count; ++s) {
-                const double t = 0.71 * ((kv_blocks + s - 1) / s) + 0.028 * (double)(tiles * s);
+            for (int s = 2; s <= 8 && 2 * s <= seen && tiles * s <= sm_count; ++s) {
+                const double t = 0.71 * ((seen + s - 1) / s) + 0.028 * (double)(tiles * s);
                 if (t < least) least = t, splits = s;
             }
         }
@@ -396,6 +371,7 @@ static int plan_prefill(const arc_sdpa_prefill_params* p, int sm_count, const Wi
     plan->ws_bytes = (plan->ws_bytes + 15) & ~(size_t)15;
     if (scanned_mask) plan->mask_bytes = (size_t)plan->q_tiles * kv_blocks * (128 * sizeof(uint4) + sizeof(uint32_t));
     if (p->block_ids && (p->mask_type != ARC_MASK_CAUSAL || p->block_ids_offset < 0)) return ARC_ERR_BAD_SHAPE;
+    if (p->sinks < 0 || (p->sinks > 0 && (p->mask_type != ARC_MASK_CAUSAL || p->block_ids))) return ARC_ERR_BAD_SHAPE;
     return ARC_OK;
 }
 
@@ -419,7 +395,8 @@ static int launch_fold(const arc_sdpa_prefill_params* p, const PrefillPlan& plan
     mp.o_stride_t = p->o_stride_t;
     mp.out_copies = kp.out_copies;
     mp.n_copies = kp.n_copies;
-    ARC_CUDA(launch_dependent(plan.splits <= 4 ? sdpa_uniform_merge_kernel<HD, 4> : sdpa_uniform_merge_kernel<HD, 8>, dim3((unsigned)((plan.rows + UMERGE_ROWS - 1) / UMERGE_ROWS)),
+    const auto kernel = p->sinks > 0 && kp.gate ? sdpa_uniform_merge_kernel<HD, 8, true> : plan.splits <= 4 ? sdpa_uniform_merge_kernel<HD, 4> : sdpa_uniform_merge_kernel<HD, 8>;
+    ARC_CUDA(launch_dependent(kernel, dim3((unsigned)((plan.rows + UMERGE_ROWS - 1) / UMERGE_ROWS)),
                               dim3(32 * UMERGE_ROWS), 0, stream, 1, mp));
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return ARC_OK;
@@ -505,6 +482,8 @@ static int launch_prefill(const arc_sdpa_prefill_params* p, const PrefillPlan& p
     kp.scale_log2 = p->scale * 1.4426950408889634f;
     kp.mask_type = p->mask_type;
     kp.window = p->window;
+    kp.sinks = sinks_of(p);
+    const bool sinks = p->sinks > 0;  // (also where they change nothing: how a gated result is rounded goes by the argument)
     kp.num_splits = plan.splits;
     kp.group = p->nq / p->nkv;
     kp.group_shift = -1;
@@ -566,7 +545,7 @@ static int launch_prefill(const arc_sdpa_prefill_params* p, const PrefillPlan& p
         cp.total_tiles = (int)single_tiles;
         auto launch_chains = [&](long long ctas) -> int {
             set_step(&cp, ctas);
-            ARC_CUDA(launch_dependent(chains_kernel(cp.gate && !split, cp.ids != nullptr, masked), dim3((unsigned)ctas), dim3(ChainsCfg::THREADS),
+            ARC_CUDA(launch_dependent(chains_kernel(cp.gate && !split, cp.ids != nullptr, masked, sinks), dim3((unsigned)ctas), dim3(ChainsCfg::THREADS),
                                       (size_t)ChainsCfg::SMEM_BYTES, stream, 1, tq, tk, tv, cp));
             g_launches.fetch_add(1, std::memory_order_relaxed);
             return ARC_OK;
@@ -582,7 +561,7 @@ static int launch_prefill(const arc_sdpa_prefill_params* p, const PrefillPlan& p
         kp.total_tiles = (int)pair_units;
         set_step(&kp, std::min(pair_units, sms));
         if ((rc = make_out_maps(&to, &tg, p)) != ARC_OK) return rc;
-        ARC_CUDA(launch_dependent(pair_kernel(kp.gate != nullptr, kp.n_copies > 0, kp.ids != nullptr), dim3((unsigned)std::min(pair_units, sms)), dim3(PairCfg::THREADS),
+        ARC_CUDA(launch_dependent(pair_kernel(kp.gate != nullptr, kp.n_copies > 0, kp.ids != nullptr, sinks), dim3((unsigned)std::min(pair_units, sms)), dim3(PairCfg::THREADS),
                                   (size_t)PairCfg::SMEM_BYTES, stream, 1, tq, tk, tv, to, tg, kp));
         g_launches.fetch_add(1, std::memory_order_relaxed);
         if (!cut_tail) return ARC_OK;
@@ -636,7 +615,7 @@ static int launch_prefill(const arc_sdpa_prefill_params* p, const PrefillPlan& p
         }
         // (a cluster is placed inside one GPC, so fewer fit than pairs / parts)
         const bool fold = split && folds_itself(p, plan.splits, wide_units(p, plan.q_tiles), ds->wide);
-        const WideKernel kernel = wide_kernel(kp.gate != nullptr, masked, fold ? 2 : split ? 1 : 0, units > ds->wide.pairs, kp.ids != nullptr);
+        const WideKernel kernel = wide_kernel(kp.gate != nullptr, masked, fold ? 2 : split ? 1 : 0, units > ds->wide.pairs, kp.ids != nullptr, sinks);
         ARC_CUDA(launch_dependent(kernel,
                                   dim3((unsigned)(2 * (split || units < ds->wide.pairs ? units : ds->wide.pairs))), dim3(WideCfg::THREADS),
                                   (size_t)WideCfg::SMEM_BYTES, stream, fold ? 2 * plan.splits : 2, tq, tk, tv, to, tg, kp));

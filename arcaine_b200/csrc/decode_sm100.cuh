@@ -93,9 +93,39 @@ __device__ __forceinline__ long long share_size(long long total, int ncta, int t
     return (per + tile_keys - 1) / tile_keys * tile_keys;
 }
 
+// What one token at the end of `len` keys sees behind a window (0x7fffffff: none): keys [0, sinks) and [lo, len), as `n`
+// slices of 16 keys, the first `ns` from key 0 on and the others from slice w0 on.  (Sinks that reach the window's first slice
+// leave no gap.)
+struct SeenKeys {
+    int len, lo, sinks, ns, w0, n;
+    __device__ __forceinline__ int slice(int i) const { return i < ns ? i : w0 + i - ns; }
+    // Bit k: key 16 s + k of the sequence is seen.
+    __device__ __forceinline__ uint32_t keys_of(int s) const {
+        const int k0 = s * 16;
+        auto below = [&](int end) { return (1u << min(max(end - k0, 0), 16)) - 1u; };  // keys in front of `end`
+        return below(len) & (~below(lo) | below(sinks));
+    }
+};
+__device__ __forceinline__ SeenKeys seen_of(int len, int window, int sinks) {
+    SeenKeys k;
+    k.len = max(0, len);
+    k.lo = window < k.len ? k.len - window : 0;
+    k.sinks = min(sinks, k.lo);
+    k.w0 = k.lo >> 4;
+    k.ns = min((k.sinks + 15) >> 4, k.w0);
+    k.n = k.len > 0 ? ((k.len - 1) >> 4) + 1 - k.w0 + k.ns : 0;
+    return k;
+}
+
 __device__ __forceinline__ float sigmoid_gate(float attn, uint16_t gate_bits) {
     const float g = bf16_bits_to_f32(gate_bits);
     return bf16_round(attn) * sigmoid(g);
+}
+
+// ONCE: rounded once, after the gate, where the reference's order of rounding (sigmoid_gate's) has no counterpart to follow.
+template <bool ONCE>
+__device__ __forceinline__ float gated(float attn, uint16_t gate_bits) {
+    return ONCE ? attn * sigmoid(bf16_bits_to_f32(gate_bits)) : sigmoid_gate(attn, gate_bits);
 }
 
 // All consumer warps of the CTA (named barrier 1; the producer warp does not take part).
@@ -734,6 +764,7 @@ struct DecodeMergeParams {
     uint32_t x_step;
     long long x_wait_cycles;  // bound of the wait for the other ranks' records
     uint32_t* fault;
+    int window, sinks;  // PAGED: which keys of a sequence are seen
 };
 
 // Layout of one rank's exchange buffer: [2 parities][world sources][rows] records of HD + 2 words, a word
@@ -767,7 +798,8 @@ constexpr int MERGE_THREADS = 256;
 // end; 64 columns a block, every load of a batch in flight with the log-sum-exps, take 3.9.
 // (Whole rows of 256: four blocks per SM, 64 sequences of 24 heads are 1536 of them.  At 128 columns the registers that
 // would take are worth more: 12 sequences of 16 heads 14.8 us, with four blocks per SM 15.6.)
-template <int HD, bool XCHG, int COLS>
+// PAGED: shares are counted in slices of 16 keys (decode_paged_sm100.cuh).
+template <int HD, bool XCHG, int COLS, bool PAGED = false>
 __global__ void __launch_bounds__(MERGE_THREADS, XCHG || COLS < 256 ? 1 : 4) sdpa_decode_merge_kernel(const DecodeMergeParams p) {
     // One row of output per block; what the block does before its one barrier every warp does for itself — where the
     // row's records are, their maximum and weights — because that is a handful of loads, while three block-wide
@@ -780,14 +812,15 @@ __global__ void __launch_bounds__(MERGE_THREADS, XCHG || COLS < 256 ? 1 : 4) sdp
     const int team = threadIdx.x / LPR, tl = threadIdx.x % LPR;
     const int lane = threadIdx.x & 31;
     // (The decode kernel released this one after its own wait for the kernels in front: the lengths are final.)
+    auto share_len = [&](int len) { return PAGED ? seen_of(len, p.window, p.sinks).n : max(0, len); };
     long long k_begin = 0, total = 0, k_len = 0;
     if (!p.kv_len) {
-        k_len = max(0, p.kv_len_uniform);
+        k_len = share_len(p.kv_len_uniform);
         k_begin = (long long)b * k_len;
         total = (long long)p.batch * k_len;
     } else {
         for (int i = lane; i < p.batch; i += 32) {
-            const int len = max(0, p.kv_len[i]);
+            const int len = share_len(p.kv_len[i]);
             total += len;
             if (i < b) k_begin += len;
             if (i == b) k_len = len;
@@ -802,7 +835,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, XCHG || COLS < 256 ? 1 : 4) sdp
     // requests for the lines the end will need
     if (p.gate && p.out && threadIdx.x < HD * 2 / 128)
         prefetch_l2(p.gate + (long long)b * p.o_stride_b + (long long)h * HD + threadIdx.x * 64);
-    const long long per = share_size(total, p.ncta, 16 * p.slices);
+    const long long per = share_size(total, p.ncta, PAGED ? p.slices : 16 * p.slices);
     const long long k_end = k_begin + k_len;
     grid_dependency_wait();                                            // from here on the partial records are read
     grid_launch_dependents();
@@ -852,6 +885,8 @@ __global__ void __launch_bounds__(MERGE_THREADS, XCHG || COLS < 256 ? 1 : 4) sdp
         for (int j = lane + 32 * MINE; j < n_rec; j += 32) mx = fmaxf(mx, lses[rec_of(j) * p.nq]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        // (PAGED: records whose log-sum-exp is no number make the row none, also where all of them are; the maximum passes them over.)
+        if (PAGED && mx == -CUDART_INF_F) mx = 0.f;
         if (mx > -CUDART_INF_F) {
             float z = 0.f;
 #pragma unroll
@@ -967,8 +1002,8 @@ __global__ void __launch_bounds__(MERGE_THREADS, XCHG || COLS < 256 ? 1 : 4) sdp
             const long long eoff = (long long)b * p.o_stride_b + (long long)h * HD + d;
             if (p.gate) {
                 const uint32_t gw = *reinterpret_cast<const uint32_t*>(p.gate + eoff);
-                a0 = sigmoid_gate(a0, (uint16_t)(gw & 0xffffu));
-                a1 = sigmoid_gate(a1, (uint16_t)(gw >> 16));
+                a0 = gated<PAGED>(a0, (uint16_t)(gw & 0xffffu));
+                a1 = gated<PAGED>(a1, (uint16_t)(gw >> 16));
             }
             *reinterpret_cast<uint32_t*>(p.out + eoff) = pack_bf16x2(a0, a1);
         }
@@ -1047,7 +1082,7 @@ __device__ __forceinline__ void load_gate_row(const UniformMergeParams& p, long 
     for (int j = 0; j < HD / 64; ++j) gw[j] = p.gate ? *reinterpret_cast<const uint32_t*>(p.gate + eoff + (threadIdx.x & 31) * (HD / 32) + 2 * j) : 0u;
 }
 
-template <int HD>
+template <int HD, bool ONCE>
 __device__ __forceinline__ void store_folded(const UniformMergeParams& p, long long row, long long eoff, float mx, float z, float (&acc)[HD / 32],
                                              const uint32_t (&gw)[HD / 64]) {
     constexpr int VPL = HD / 32;
@@ -1067,8 +1102,8 @@ __device__ __forceinline__ void store_folded(const UniformMergeParams& p, long l
         for (int j = 0; j < VPL / 2; ++j) {
             float a0 = acc[2 * j], a1 = acc[2 * j + 1];
             if (p.gate) {
-                a0 = sigmoid_gate(a0, (uint16_t)(gw[j] & 0xffffu));
-                a1 = sigmoid_gate(a1, (uint16_t)(gw[j] >> 16));
+                a0 = gated<ONCE>(a0, (uint16_t)(gw[j] & 0xffffu));
+                a1 = gated<ONCE>(a1, (uint16_t)(gw[j] >> 16));
             }
             packed[j] = pack_bf16x2(a0, a1);
         }
@@ -1085,7 +1120,7 @@ __device__ __forceinline__ void store_folded(const UniformMergeParams& p, long l
 // merge of six parts of 2048 rows took 2.6 us more than that of four.)
 constexpr int UMERGE_ROWS = 8;  // rows per block
 
-template <int HD, int U>
+template <int HD, int U, bool ONCE = false>
 __global__ void __launch_bounds__(32 * UMERGE_ROWS) sdpa_uniform_merge_kernel(const UniformMergeParams p) {
     const long long row = (long long)blockIdx.x * UMERGE_ROWS + (threadIdx.x >> 5);
     long long eoff = row * HD;
@@ -1108,11 +1143,11 @@ __global__ void __launch_bounds__(32 * UMERGE_ROWS) sdpa_uniform_merge_kernel(co
         load_parts<HD, U>(p, row, i0, li, ov);
         fold_parts<HD, U>(li, ov, mx, z, acc);
     }
-    store_folded<HD>(p, row, eoff, mx, z, acc, gw);
+    store_folded<HD, ONCE>(p, row, eoff, mx, z, acc, gw);
 }
 
 // a[i] = bf16(f32(a[i]) * sigmoid(f32(gate[i]))) : src/modeling/qwen3_5_moe/kernels.hpp:80-88
-__global__ void mul_sigmoid_kernel(uint16_t* a, const uint16_t* gate, long long n) {
+static __global__ void mul_sigmoid_kernel(uint16_t* a, const uint16_t* gate, long long n) {
     grid_dependency_wait();
     grid_launch_dependents();
     const long long stride = (long long)gridDim.x * blockDim.x;

@@ -46,10 +46,11 @@ struct ChainsCfg {
 // One tile (or a part of its key range): key blocks [lo, hi), block lo + i in chain i & 1.
 struct ChainsWork {
     int q0, h, b, kvh, lo, hi, part;
+    int gap;  // SINKS (key_block)
     __device__ __forceinline__ int blocks() const { return hi - lo; }
 };
 
-template <bool VISION>
+template <bool VISION, bool SINKS>
 __device__ __forceinline__ ChainsWork decode_chains(const PrefillParams& p, const TileCursor& cur) {
     ChainsWork t;
     t.b = cur.z;
@@ -62,6 +63,10 @@ __device__ __forceinline__ ChainsWork decode_chains(const PrefillParams& p, cons
     t.kvh = p.group_shift >= 0 ? (cur.h >> p.group_shift) : cur.h / p.group;
     t.q0 = cur.qt * ChainsCfg::BM;
     tile_blocks<VISION>(p, t.q0, t.lo, t.hi);
+    if constexpr (SINKS) {
+        t.gap = t.lo;
+        t.lo = sinks_begin(p, t.gap);
+    }
     if (p.num_splits > 1) {
         const int n = t.hi - t.lo;
         t.hi = t.lo + n * (t.part + 1) / p.num_splits;
@@ -111,9 +116,10 @@ __device__ __forceinline__ uint32_t gate_pair(uint32_t attn, uint32_t gate) {
 // Every softmax warp executes the same number of them per tile, whatever happened to its waits.
 __device__ __forceinline__ void row_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
 
-// VISION: causal with vision blocks (p.ids).  MASKED: an additive mask.  num_splits > 1: a unit is a part of the key range,
+// VISION: causal with vision blocks (p.ids).  MASKED: an additive mask.  SINKS: the first p.sinks keys stay visible behind the window; gated
+// results are rounded once.  num_splits > 1: a unit is a part of the key range,
 // whose normalised rows go to the partial records as f32 with their log-sum-exp.
-template <bool GATE, bool VISION, bool MASKED>
+template <bool GATE, bool VISION, bool MASKED, bool SINKS = false>
 __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
     sdpa_prefill_chains_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                                const __grid_constant__ CUtensorMap tm_v, const PrefillParams p) {
@@ -179,28 +185,29 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
     TileCursor cur;  // (with its divisions, ahead of the wait)
     cur.init(p);
     ChainsWork tw{};
-    if (!VISION) tw = decode_chains<false>(p, cur);
+    if (!VISION) tw = decode_chains<false, SINKS>(p, cur);
     __syncthreads();
     // Up to here nothing depends on the kernels in front; everything below may.  (The tail of a two-tile launch runs beside
     // that launch, which let it start only when the kernels before it had completed.)
     if (p.tail_base < 0) grid_dependency_wait();
     grid_launch_dependents();
     if (threadIdx.x == 0) *abort_slot = *reinterpret_cast<volatile uint32_t*>(p.fault) != 0u ? 1u : 0u;
-    if (VISION) tw = decode_chains<true>(p, cur);  // (whole warps)
+    if (VISION) tw = decode_chains<true, SINKS>(p, cur);  // (whole warps)
+    auto key_of = [&](int j) { return (SINKS ? key_block(p, j, tw.gap) : j) * C::BN; };  // first key of the tile's block j
     auto load_first = [&](int st) {  // Q and the first K
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             if (lane == 0) mbar_arrive_expect_tx(&first[c], 2 * C::CHUNK_BYTES);
             __syncwarp();
             tma_load_4d_warp(sQ + c * C::CHUNK_BYTES, &tm_q, &first[c], c * 64, tw.h, tw.q0, tw.b);
-            tma_load_4d_warp(sK + st * C::TILE_BYTES + c * C::CHUNK_BYTES, &tm_k, &first[c], c * 64, tw.kvh, tw.lo * C::BN, tw.b);
+            tma_load_4d_warp(sK + st * C::TILE_BYTES + c * C::CHUNK_BYTES, &tm_k, &first[c], c * 64, tw.kvh, key_of(tw.lo), tw.b);
         }
     };
     auto load = [&](uint8_t* dst, const void* tm, uint64_t* bar, int i) {  // K or V of the tile's block i
         if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE_BYTES);
         __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) tma_load_4d_warp(dst + c * C::CHUNK_BYTES, tm, bar, c * 64, tw.kvh, (tw.lo + i) * C::BN, tw.b);
+        for (int c = 0; c < 2; ++c) tma_load_4d_warp(dst + c * C::CHUNK_BYTES, tm, bar, c * 64, tw.kvh, key_of(tw.lo + i), tw.b);
     };
     // The first tile's Q, its first two K and its first V
     const int ahead_k = min(tw.blocks(), 2), ahead_v = min(tw.blocks(), 1);
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
     const int total_tiles = aborted ? 0 : p.total_tiles;  // a status is set: walk an empty list
     auto next_tile = [&]() {
         cur.advance(p);
-        if (cur.w < total_tiles) tw = decode_chains<VISION>(p, cur);
+        if (cur.w < total_tiles) tw = decode_chains<VISION, SINKS>(p, cur);
     };
 
     if (warp >= C::PRODUCER_WARP) {
@@ -406,11 +413,12 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
                 if (row_lo > row_hi) row_lo = row_hi;
             }
             const RowMask rm{row_lo, row_hi};
+            const int row_sinks = SINKS ? min(p.sinks, row_hi) : 0;
 
             float m = -CUDART_INF_F;  // running max of the chain, log2 domain, possibly stale by <= 8
             float l = 0.f;            // its sum
             for (int j = tw.lo + s; ok && j < tw.hi; j += 2, ++g) {
-                const int kc = j * C::BN;
+                const int kc = key_of(j);
                 uint32_t bits[4];
                 bool values = false;
                 if (MASKED) values = read_mask_bits(p.mask, t - lane, p.seq, kc, p.kv_len, bits);
@@ -426,13 +434,14 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
                     add_mask_values(tS, p.mask, t, p.seq, kc, p.kv_len, sl);
                     bl = 1.0f, bl2 = pack_f32x2(1.0f, 1.0f);
                 }
-                const bool full = !MASKED && __all_sync(0xffffffffu, rm.lo <= kc && kc + C::BN <= rm.hi);
+                const bool full = !MASKED && __all_sync(0xffffffffu, (rm.lo <= kc && kc + C::BN <= rm.hi) || (SINKS && kc + C::BN <= row_sinks));
                 float mr[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
                 auto mask = [&](uint32_t (&v)[32], int c) {
                     if constexpr (MASKED) {
                         if (!values) select_chunk(v, bits[c]);
-                    } else {
-                        if (!full) mask_chunk(v, kc + c * 32, rm);  // window edge, diagonal, ragged end
+                    } else if (!full) {  // window edge, diagonal, ragged end
+                        if constexpr (SINKS) mask_chunk(v, kc + c * 32, rm, row_sinks);
+                        else mask_chunk(v, kc + c * 32, rm);
                     }
                 };
                 tmem_ld32(tS, s0);
@@ -531,6 +540,15 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
             // could go.
             __syncwarp();  // (the tile before has left the buffer)
             const uint32_t at = smem_u32(out_buf) + lane * 128;
+            const int row0 = quarter * 32 + (lane >> 3), col = (lane & 7) * 8;  // this lane's first row, its columns of the warp's 64
+            const long long out0 = tw.b * p.o_stride_b + (tw.q0 + row0) * p.o_stride_t + (long long)tw.h * HD + s * 64 + col;
+            if (GATE && SINKS && !split) {  // the gate's values where the results go, for their rows' lanes
+                for (int i = 0; i < 8 && tw.q0 + row0 + 4 * i < p.seq; ++i) {
+                    const int rr = (lane >> 3) + 4 * i;
+                    *reinterpret_cast<uint4*>(out_buf + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)) = *reinterpret_cast<const uint4*>(p.gate + out0 + 4 * i * p.o_stride_t);
+                }
+                __syncwarp();
+            }
             uint32_t a[32], b[32];
             auto fetch = [&](int c) {
                 tmem_ld32(tO + s * 64 + c * 32, a);
@@ -560,6 +578,20 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
                     }
                     continue;
                 }
+                if constexpr (GATE && SINKS) {
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t g[4];
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(g[0]), "=r"(g[1]), "=r"(g[2]), "=r"(g[3]) : "r"(at + (((4 * c + i) ^ (lane & 7)) << 4)));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float gate = sigmoid(__uint_as_float(e & 1 ? g[e / 2] & 0xffff0000u : g[e / 2] << 16));
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (k == i) o[8 * k + e] *= gate;
+                        }
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((4 * c + i) ^ (lane & 7)) << 4)), "r"(pack_bf16x2(o[8 * i], o[8 * i + 1])),
@@ -568,18 +600,17 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
             }
             if (split) continue;
             __syncwarp();
-            const int row0 = quarter * 32 + (lane >> 3), col = (lane & 7) * 8;  // this lane's first row, its columns of the warp's 64
-            const long long out0 = tw.b * p.o_stride_b + (tw.q0 + row0) * p.o_stride_t + (long long)tw.h * HD + s * 64 + col;
             // (Gated two at a time: eight, 64 sigmoids of code that is fetched cold, cost a call of 100 rows 0.1 us less from warm caches
             // and 2.4 more from cold ones: 12.3 and 9.9.)
-            constexpr int AT_ONCE = GATE ? 2 : 8;
+            constexpr bool GATE_LATE = GATE && !SINKS;
+            constexpr int AT_ONCE = GATE_LATE ? 2 : 8;
 #pragma unroll AT_ONCE
             for (int i = 0; i < 8; ++i) {
                 if (tw.q0 + row0 + 4 * i >= p.seq) break;
                 const int rr = (lane >> 3) + 4 * i;
                 uint4 v = *reinterpret_cast<const uint4*>(out_buf + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
                 const long long to = out0 + 4 * i * p.o_stride_t;
-                if (GATE) {  // (in L2 since the tile began)
+                if (GATE_LATE) {  // (in L2 since the tile began)
                     const uint4 g4 = *reinterpret_cast<const uint4*>(p.gate + to);
                     v.x = gate_pair(v.x, g4.x), v.y = gate_pair(v.y, g4.y), v.z = gate_pair(v.z, g4.z), v.w = gate_pair(v.w, g4.w);
                 }

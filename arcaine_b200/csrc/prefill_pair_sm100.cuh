@@ -83,6 +83,7 @@ struct PairWork {
     int b, kvh;
     int lo[2], hi[2];
     int ulo, uhi;  // union of the two ranges (contiguous)
+    int gap;  // SINKS (key_block)
     bool live[2];  // the tile has rows below seq
     // Selected without dynamic indexing, so the struct stays in registers.
     __device__ __forceinline__ int q0_of(int s) const { return s ? q0[1] : q0[0]; }
@@ -150,9 +151,16 @@ __device__ __forceinline__ void tile_blocks(const PrefillParams& p, int qs, int&
     if (blk_hi < blk_lo) blk_hi = blk_lo;
 }
 
+// Keys that stay visible behind a window (sinks): their blocks go in front of the window's, which begin at block `lo`, and all roles
+// count them as blocks right ahead of it, from sinks_begin(lo) on.  So nothing but loads and masks knows that they are elsewhere.
+// (A tile that sees nothing has lo = 0.)
+__device__ __forceinline__ int sinks_begin(const PrefillParams& p, int lo) { return lo - min((p.sinks + 127) >> 7, lo); }
+// The keys' block that is block j of a tile whose window begins at block `gap`.
+__device__ __forceinline__ int key_block(const PrefillParams& p, int j, int gap) { return j < gap ? j - sinks_begin(p, gap) : j; }
+
 // Every role runs this once per unit, from code that has long left the instruction caches by
 // then, so it is kept short: one division at most, and nothing computed twice.
-template <bool VISION>
+template <bool VISION, bool SINKS>
 __device__ __forceinline__ PairWork decode_pair(const PrefillParams& p, const TileCursor& cur) {
     PairWork t;
     t.b = cur.z;
@@ -185,6 +193,13 @@ __device__ __forceinline__ PairWork decode_pair(const PrefillParams& p, const Ti
             }
     }
     if (t.uhi == 0) t.ulo = 0;
+    if constexpr (SINKS) {  // (the second tile's blocks, too, from the first one's window on: what it does not see is masked)
+        t.gap = t.ulo;
+        t.ulo = sinks_begin(p, t.gap);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            if (t.hi[s] > t.lo[s]) t.lo[s] = t.ulo;
+    }
     return t;
 }
 
@@ -193,6 +208,14 @@ __device__ __forceinline__ PairWork decode_pair(const PrefillParams& p, const Ti
 __device__ __forceinline__ void mask_chunk(uint32_t (&v)[32], int key0, const RowMask& rm) {
     const int lo = min(max(rm.lo - key0, 0), 32), hi = min(max(rm.hi - key0, 0), 32);
     const uint32_t vis = (uint32_t)((1ull << hi) - (1ull << lo));  // bits [lo, hi); lo > hi cannot be (a span is never negative)
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = (vis >> e) & 1u ? v[e] : 0xff800000u;
+}
+
+// The same where keys [0, sinks) are visible, too.
+__device__ __forceinline__ void mask_chunk(uint32_t (&v)[32], int key0, const RowMask& rm, int sinks) {
+    const int lo = min(max(rm.lo - key0, 0), 32), hi = min(max(rm.hi - key0, 0), 32), first = min(max(sinks - key0, 0), 32);
+    const uint32_t vis = (uint32_t)(((1ull << hi) - (1ull << lo)) | ((1ull << first) - 1ull));
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] = (vis >> e) & 1u ? v[e] : 0xff800000u;
 }
@@ -292,7 +315,8 @@ __device__ __forceinline__ void stage_send(const OutStage& s, const void* tm_out
 // Turn k: the accumulator's values times `inv`, gated, as bf16 into the buffer (and into w8 for the caller); after a
 // round's last turn the round is sent off.  taken(): called once acc has been used, so that the next turn's values
 // can be on their way while this turn's are gated.
-template <bool GATE, typename F, int N>
+// ONCE: rounded after the gate only.
+template <bool GATE, bool ONCE = false, typename F, int N>
 __device__ __forceinline__ void stage_turn(const OutStage& s, const void* tm_out, int lane, int k, const uint32_t (&acc)[N], float inv,
                                            uint32_t (&w8)[N / 2], F&& taken) {
     constexpr int TURNS = 64 / N;
@@ -306,11 +330,15 @@ __device__ __forceinline__ void stage_turn(const OutStage& s, const void* tm_out
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gw[4 * i]), "=r"(gw[4 * i + 1]), "=r"(gw[4 * i + 2]), "=r"(gw[4 * i + 3]) : "r"(at[i]));
     }
 #pragma unroll
-    for (int u = 0; u < N / 2; ++u) w8[u] = pack_bf16x2(__uint_as_float(acc[2 * u]) * inv, __uint_as_float(acc[2 * u + 1]) * inv);
+    for (int u = 0; u < N / 2; ++u) {
+        float a0 = __uint_as_float(acc[2 * u]) * inv, a1 = __uint_as_float(acc[2 * u + 1]) * inv;
+        if constexpr (GATE && ONCE) a0 *= sigmoid(__uint_as_float(gw[u] << 16)), a1 *= sigmoid(__uint_as_float(gw[u] & 0xffff0000u));
+        w8[u] = pack_bf16x2(a0, a1);
+    }
     taken();
 #pragma unroll
     for (int i = 0; i < N / 8; ++i) {
-        if (GATE) {
+        if (GATE && !ONCE) {
             // bf16(attention) * sigmoid(gate): the rounding order of the two-launch form
 #pragma unroll
             for (int u = 4 * i; u < 4 * i + 4; ++u) {
@@ -326,8 +354,9 @@ __device__ __forceinline__ void stage_turn(const OutStage& s, const void* tm_out
 
 // The gated epilogue and the one that also stores copies of the output are instances of their own: code the
 // common kernel does not carry.
-// VISION: causal with vision blocks (p.ids).
-template <bool GATE, bool COPIES, bool VISION = false>
+// VISION: causal with vision blocks (p.ids).  SINKS: the first p.sinks keys stay visible behind the window; gated results are
+// rounded once.
+template <bool GATE, bool COPIES, bool VISION = false, bool SINKS = false>
 __global__ void __launch_bounds__(PairCfg::THREADS, 1)
     sdpa_prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
@@ -433,13 +462,13 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
             auto load = [&](uint8_t* dst, const void* tm, uint64_t* bar, const PairWork& pw, int j) {
 #pragma unroll
                 for (int c = 0; c < C::CH; ++c)
-                    tma_load_4d_warp(dst + c * C::CHUNK_BYTES, tm, bar, c * 64, pw.kvh, j * C::BN, pw.b);
+                    tma_load_4d_warp(dst + c * C::CHUNK_BYTES, tm, bar, c * 64, pw.kvh, (SINKS ? key_block(p, j, pw.gap) : j) * C::BN, pw.b);
             };
             TileCursor cur = *cursor;
             PairWork last{};  // unit and index of the block requested last
             int last_j = 0;
             for (; ok && cur.w < total_tiles; cur.advance(p)) {
-                const PairWork pw = decode_pair<VISION>(p, cur);
+                const PairWork pw = decode_pair<VISION, SINKS>(p, cur);
                 for (int j = pw.ulo; ok && j < pw.uhi; ++j, ++r) {
                     if (r == 0) {
                         if (lane == 0) mbar_arrive_expect_tx(k_first, C::TILE_BYTES);
@@ -486,7 +515,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                 bool ok = true;
                 TileCursor cur = *cursor;
                 for (; ok && cur.w < total_tiles; cur.advance(p)) {
-                    const PairWork pw = decode_pair<VISION>(p, cur);
+                    const PairWork pw = decode_pair<VISION, SINKS>(p, cur);
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         if (pw.hi[s] == pw.lo[s]) continue;
@@ -510,7 +539,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                     TileCursor nx = cur;
                     nx.advance(p);
                     if (ok && !VISION && nx.w < total_tiles) {
-                        const PairWork pn = decode_pair<false>(p, nx);
+                        const PairWork pn = decode_pair<false, SINKS>(p, nx);
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
                             if (pn.hi[s] == pn.lo[s]) continue;
@@ -538,7 +567,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
             bool ok = true;
             TileCursor cur = *cursor;
             for (; ok && cur.w < total_tiles; cur.advance(p)) {
-                const PairWork pw = decode_pair<VISION>(p, cur);
+                const PairWork pw = decode_pair<VISION, SINKS>(p, cur);
                 for (int j = pw.ulo; ok && j < pw.uhi; ++j, ++r) {
                     if (!mbar_wait_inline(r ? &kv_full[(r - 1) & 1] : k_first, r ? ((r - 1) >> 1) & 1 : 0)) {
                         if (lane == 0) report_fault(p.fault, FAULT_WAIT_K, r);
@@ -582,7 +611,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
             bool ok = true;
             TileCursor cur = *cursor;
             for (; ok && cur.w < total_tiles; cur.advance(p)) {
-                const PairWork pw = decode_pair<VISION>(p, cur);
+                const PairWork pw = decode_pair<VISION, SINKS>(p, cur);
                 for (int j = pw.ulo; ok && j < pw.uhi; ++j, ++r) {
                     if (!mbar_wait_inline(&kv_full[r & 1], (r >> 1) & 1)) {
                         if (lane == 0) report_fault(p.fault, FAULT_WAIT_V, r);
@@ -643,7 +672,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
         OutStage stage{sOut + quarter * STAGE_WARP_BYTES, &gate_bar[2 * quarter], 0u, 0, 0, 0, 0, HD / 64};
         TileCursor cur = *cursor;
         for (; ok && cur.w < total_tiles; cur.advance(p)) {
-            const PairWork pw = decode_pair<VISION>(p, cur);
+            const PairWork pw = decode_pair<VISION, SINKS>(p, cur);
 #pragma unroll 1
             for (int s = 0; s < 2 && ok; ++s) {
                 const int t0 = pw.q0_of(s) + quarter * 32, t = t0 + lane, h = pw.h_of(s);
@@ -699,7 +728,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                     };
                     if (!warp_store) next();
                     if (warp_store) {
-                        stage_turn<GATE>(stage, &tm_out, lane, c, wa, inv, w8, next);
+                        stage_turn<GATE, SINKS>(stage, &tm_out, lane, c, wa, inv, w8, next);
                         if (COPIES && store) {
                             for (int k = 0; k < p.n_copies; ++k) {
                                 uint4* d4 = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out_copies[k]) + eoff + c * SC);
@@ -736,7 +765,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
 
         TileCursor cur = *cursor;
         for (; ok && cur.w < total_tiles; cur.advance(p)) {
-            const PairWork pw = decode_pair<VISION>(p, cur);
+            const PairWork pw = decode_pair<VISION, SINKS>(p, cur);
             if (pw.uhi == pw.ulo) continue;
             const int t = pw.q0_of(s) + r;
             const int lo = pw.lo_of(s), hi = pw.hi_of(s);
@@ -749,18 +778,23 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                 if (row_lo > row_hi) row_lo = row_hi;
             }
             const RowMask rm{row_lo, row_hi};
+            const int row_sinks = SINKS ? min(p.sinks, row_hi) : 0;
+            auto mask = [&](uint32_t (&v)[32], int key0) {
+                if constexpr (SINKS) mask_chunk(v, key0, rm, row_sinks);
+                else mask_chunk(v, key0, rm);
+            };
 
             float m = -CUDART_INF_F;  // running max, log2 domain, possibly stale by <= 8
             float l = 0.f;            // row sum
             for (int j = lo; j < hi; ++j, ++g) {
-                const int kc = j * C::BN;
+                const int kc = (SINKS ? key_block(p, j, pw.gap) : j) * C::BN;
                 if (!mbar_wait_warp<3>(&s_full[s], g & 1)) {
                     report_fault(p.fault, FAULT_WAIT_S, g);
                     ok = false;
                     break;
                 }
                 tc_fence_after_sync();
-                const bool full = __all_sync(0xffffffffu, rm.lo <= kc && kc + C::BN <= rm.hi);
+                const bool full = __all_sync(0xffffffffu, (rm.lo <= kc && kc + C::BN <= rm.hi) || (SINKS && kc + C::BN <= row_sinks));
                 float mr[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
                 tmem_ld32(tS, s0);
                 tmem_ld32(tS + 32, s1);
@@ -768,8 +802,8 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                 tmem_ld32(tS + 64, s2);  // lands while the maximum of the first half is taken
                 tmem_ld32(tS + 96, s3);
                 if (!full) {  // window edge, diagonal, ragged end (two blocks in nine with a 1024-key window)
-                    mask_chunk(s0, kc, rm);
-                    mask_chunk(s1, kc + 32, rm);
+                    mask(s0, kc);
+                    mask(s1, kc + 32);
                 }
                 chunk_max(s0, mr);
                 chunk_max(s1, mr);
@@ -777,8 +811,8 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                 tc_fence_before_sync();
                 mbar_arrive_warp(s_free);  // the buffer may take the other pipeline's scores
                 if (!full) {
-                    mask_chunk(s2, kc + 64, rm);
-                    mask_chunk(s3, kc + 96, rm);
+                    mask(s2, kc + 64);
+                    mask(s3, kc + 96);
                 }
                 chunk_max(s2, mr);
                 chunk_max(s3, mr);

@@ -56,6 +56,7 @@ struct WideCfg {
 struct WideWork {
     int q0, h, b, kvh, lo, hi;
     int part;  // of the key range
+    int gap;  // SINKS (key_block)
 };
 
 // ---------------------------------------------------------------------------
@@ -247,12 +248,16 @@ __device__ __forceinline__ WideWork wide_place(const PrefillParams& p, const Wid
     return t;
 }
 
-template <bool MASKED, bool SPLIT, bool VISION>
+template <bool MASKED, bool SPLIT, bool VISION, bool SINKS>
 __device__ __forceinline__ void wide_find_blocks(const PrefillParams& p, int rank, WideWork& t) {
     const int rows = p.head_pair ? WideCfg::BM : 2 * WideCfg::BM;  // tokens of the unit
     const int q0 = p.head_pair ? t.q0 : t.q0 - rank * WideCfg::BM;
     if constexpr (MASKED) masked_blocks(p, q0 >> 7, min(q0 + rows, p.seq + 127) >> 7, t.lo, t.hi);
     else wide_blocks<VISION>(p, q0, q0 + rows - 1, t.lo, t.hi);
+    if constexpr (SINKS) {
+        t.gap = t.lo;
+        t.lo = sinks_begin(p, t.gap);
+    }
     if (SPLIT) {
         const int lo = t.lo, n = t.hi - t.lo;
         t.lo = lo + n * t.part / p.num_splits;
@@ -278,7 +283,8 @@ __device__ __forceinline__ void wide_find_blocks(const PrefillParams& p, int ran
 // 16/8 heads with three images 24.4 -> 23.2 us.)
 // ONE: not SEVERAL, one unit a pair.  The walks are then left out of every role; small calls waited for them (161 queries of 24/4 heads over
 // 202 keys 8.28 -> 7.74 us, gated 9.92 -> 9.33; 64 of 16/8 over 64 6.81 -> 6.29).
-template <bool GATE, bool MASKED, int SPLIT = 0, bool SEVERAL = false, bool VISION = false>
+// SINKS: the first p.sinks keys stay visible behind the window; gated results are rounded once.
+template <bool GATE, bool MASKED, int SPLIT = 0, bool SEVERAL = false, bool VISION = false, bool SINKS = false>
 __global__ void __launch_bounds__(WideCfg::THREADS, 1)
     sdpa_prefill_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
@@ -345,7 +351,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
     WideWork w_first{};
     if (warp == C::EPILOGUE_WARP) {
         w_first = wide_place<SPLIT != 0>(p, Cursor(p), rank);
-        if (!blocks_in_memory) wide_find_blocks<MASKED, SPLIT != 0, VISION>(p, rank, w_first);
+        if (!blocks_in_memory) wide_find_blocks<MASKED, SPLIT != 0, VISION, SINKS>(p, rank, w_first);
         if (lane == 0) *first_unit = w_first;
     }
     cluster_sync_all();  // both CTAs' barriers exist before anyone arrives on the other's
@@ -353,6 +359,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
     grid_dependency_wait();
     grid_launch_dependents();
     if (threadIdx.x == 0) *abort_slot = *reinterpret_cast<volatile uint32_t*>(p.fault) != 0u ? 1u : 0u;
+    auto key_of = [&](const WideWork& w, int j) { return (SINKS ? key_block(p, j, w.gap) : j) * C::BN; };  // first key of the unit's block j
     // Q and the first K of a unit, 64 head-dim columns after 64; K or V of another block
     auto load_first = [&](const WideWork& w, int st) {
         const uint32_t b_first = map_to_cta(smem_u32(first), lead);
@@ -361,7 +368,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
             if (leader && lane == 0) mbar_arrive_expect_tx(&first[c], 2 * (C::Q_CHUNK + C::K_CHUNK));
             __syncwarp();
             tma_load_4d_pair(sQ + c * C::Q_CHUNK, &tm_q, b_first + c * 8, c * 64, w.h, w.q0, w.b);
-            tma_load_4d_pair(sK + st * C::K_BYTES + c * C::K_CHUNK, &tm_k, b_first + c * 8, c * 64, w.kvh, w.lo * C::BN + rank * 64, w.b);
+            tma_load_4d_pair(sK + st * C::K_BYTES + c * C::K_CHUNK, &tm_k, b_first + c * 8, c * 64, w.kvh, key_of(w, w.lo) + rank * 64, w.b);
         }
     };
     auto load_k = [&](const WideWork& w, int j, int st) {
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-            tma_load_4d_pair(sK + st * C::K_BYTES + c * C::K_CHUNK, &tm_k, b_k + st * 8, c * 64, w.kvh, j * C::BN + rank * 64, w.b);
+            tma_load_4d_pair(sK + st * C::K_BYTES + c * C::K_CHUNK, &tm_k, b_k + st * 8, c * 64, w.kvh, key_of(w, j) + rank * 64, w.b);
     };
     auto load_v = [&](const WideWork& w, int j, int st) {
         const uint32_t b_v = map_to_cta(smem_u32(v_full), lead);
@@ -378,7 +385,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-            tma_load_4d_pair(sV + st * C::V_BYTES + c * C::V_CHUNK, &tm_v, b_v + st * 8, rank * 128 + c * 64, w.kvh, j * C::BN, w.b);
+            tma_load_4d_pair(sV + st * C::V_BYTES + c * C::V_CHUNK, &tm_v, b_v + st * 8, rank * 128 + c * 64, w.kvh, key_of(w, j), w.b);
     };
     // The first unit's first blocks are asked for before the status word has been looked at (another 500 clk).
     int ahead_k = 0, ahead_v = 0;
@@ -388,7 +395,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
     if (warp == C::PRODUCER_WARP) {
         w_first = *first_unit;
         if (blocks_in_memory) {
-            wide_find_blocks<MASKED, SPLIT != 0, VISION>(p, rank, w_first);
+            wide_find_blocks<MASKED, SPLIT != 0, VISION, SINKS>(p, rank, w_first);
             if (lane == 0) *first_unit = w_first;
         }
         __syncwarp();
@@ -410,7 +417,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
     auto unit_at = [&](const Cursor& cur) {
         if (ONE || cur.i == 0) return *first_unit;
         WideWork w = wide_place<SPLIT != 0>(p, cur, rank);
-        wide_find_blocks<MASKED, SPLIT != 0, VISION>(p, rank, w);
+        wide_find_blocks<MASKED, SPLIT != 0, VISION, SINKS>(p, rank, w);
         return w;
     };
 
@@ -517,7 +524,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
             };
             if (!warp_store) next();
             if (warp_store) {
-                stage_turn<GATE>(stage, &tm_out, lane, c, wa, inv, w8, next);
+                stage_turn<GATE, SINKS>(stage, &tm_out, lane, c, wa, inv, w8, next);
                 store_copies(stage, w8, SC / 2, stage.col0 + c * SC);
             }
         }
@@ -842,8 +849,14 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                 if (row_lo > row_hi) row_lo = row_hi;
             }
             const RowMask rm{row_lo, row_hi};
+            const int row_sinks = SINKS ? min(p.sinks, row_hi) : 0;
+            auto mask = [&](uint32_t (&v)[32], int key0) {
+                if constexpr (SINKS) mask_chunk(v, key0, rm, row_sinks);
+                else mask_chunk(v, key0, rm);
+            };
             float m = -CUDART_INF_F;  // running max, log2 domain, possibly stale by <= 8
             float l = 0.f;            // row sum
+            [[maybe_unused]] float rounded = 0.f;  // SINKS: what rounding the blocks' largest probabilities has added to it
             // (MASKED: a block's class is asked for a block ahead, its bits before its scores are waited for)
             auto class_of = [&](int j) -> uint32_t {
                 return MASKED && w.q0 < p.seq && j < w.hi
@@ -856,7 +869,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                 const bool by_bits = (cls & (MASK_HIDDEN | MASK_VALUES)) == MASK_HIDDEN;
                 uint4 bits = make_uint4(0u, 0u, 0u, 0u);
                 if (MASKED && by_bits) bits = p.mask_bits[((long long)(w.q0 >> 7) * p.mask_blocks + j) * 128 + r];
-                const int kc = j * C::BN, st = g & 1;
+                const int kc = key_of(w, j), st = g & 1;
                 const uint32_t tS = tmem_base + lane_sel + C::COL_S + st * 128;
                 if (!mbar_wait_inline(&s_full[st], (g >> 1) & 1)) {
                     if (lane == 0) report_fault(p.fault, FAULT_WAIT_S, g);
@@ -882,11 +895,11 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                         select_chunk(s2, bits.z);
                         select_chunk(s3, bits.w);
                     }
-                } else if (!__all_sync(0xffffffffu, rm.lo <= kc && kc + C::BN <= rm.hi)) {  // window edge, diagonal, ragged end
-                    mask_chunk(s0, kc, rm);
-                    mask_chunk(s1, kc + 32, rm);
-                    mask_chunk(s2, kc + 64, rm);
-                    mask_chunk(s3, kc + 96, rm);
+                } else if (!__all_sync(0xffffffffu, (rm.lo <= kc && kc + C::BN <= rm.hi) || (SINKS && kc + C::BN <= row_sinks))) {  // window edge, diagonal, ragged end
+                    mask(s0, kc);
+                    mask(s1, kc + 32);
+                    mask(s2, kc + 64);
+                    mask(s3, kc + 96);
                 }
                 float mr[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
                 chunk_max(s0, mr);
@@ -919,6 +932,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                     }
                     tmem_wait_st();
                     l *= alpha;
+                    if (SINKS) rounded *= alpha;
                     if (need) m = m_new;
                 }
                 // Probabilities as bf16, packed over the first 64 of the block's score columns; row sum in fp32.
@@ -930,6 +944,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                 // one key dominates would otherwise be off by that rounding whenever m is stale (2^-9, as much as the output's own).
                 const float p_top = fast_exp2(fmaf(top, bl, -m_eff));
                 l += bf16_round(p_top) - p_top;
+                if (SINKS) rounded += bf16_round(p_top) - p_top;
                 uint32_t pk[16];
                 exp_chunk(s0, pk, ls2, bl2, nm2);
                 tmem_st16(tS, pk);
@@ -953,11 +968,13 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
             }
             if (ok) {
                 fin_vals[(n & 3) * 128 + r] = l;
+                // (SINKS: the log-sum-exp is that of the sum as it is; with the roundings, which the others keep in it, it is off by 1e-4.)
+                const float z = SINKS ? l - rounded : l;
                 // (SPLIT: the place in the output is read again, not kept in registers through the blocks)
                 const WideWork u = SPLIT ? *first_unit : w;
                 float* lse = SPLIT == 1 ? p.part_lse + (long long)u.part * p.batch * p.seq * p.nq : SPLIT == 2 ? p.part_lse : p.out_lse;
                 if (lse && u.q0 + r < p.seq)
-                    lse[SPLIT == 2 ? record_row(u, u.part) + r : ((long long)u.b * p.seq + u.q0 + r) * p.nq + u.h] = l > 0.f ? (m + fast_log2(l)) * 0.6931471805599453f : -CUDART_INF_F;
+                    lse[SPLIT == 2 ? record_row(u, u.part) + r : ((long long)u.b * p.seq + u.q0 + r) * p.nq + u.h] = z > 0.f ? (m + fast_log2(z)) * 0.6931471805599453f : -CUDART_INF_F;
                 mbar_arrive_warp(&fin[n & 3]);
                 ++n;
                 if constexpr (GATE && SPLIT == 0) {
@@ -1036,7 +1053,10 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
             // of them held beside the others' values, and through the barrier, made the kernel spill.)  Out through shared memory
             // (Q, K and V are through), so that a store writes whole rows of the warp's columns: a thread's own 16 bytes at a time
             // took 1800 clk.
-            constexpr int PITCH = TAKES * GROUP * 2 + 16;
+            // (ONCE: as f32, to be rounded behind the gate.)
+            constexpr bool ONCE = GATE && SINKS;
+            constexpr int PITCH = TAKES * GROUP * (ONCE ? 4 : 2) + 16;
+            static_assert(8 * 32 * PITCH <= C::Q_BYTES + C::STAGES * (C::K_BYTES + C::V_BYTES), "in Q, K and V");
             const uint32_t tile = smem_u32(smem) + warp * 32 * PITCH;
             const long long eoff = w.b * p.o_stride_b + w.q0 * p.o_stride_t + (long long)w.h * HD + my_first * GROUP;
             const uint32_t tO = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + C::COL_O + my_first * GROUP;
@@ -1062,12 +1082,18 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                         }
                     }
                 }
-                uint32_t o[GROUP / 2];
+                if constexpr (ONCE) {
 #pragma unroll
-                for (int i = 0; i < GROUP / 2; ++i) o[i] = pack_bf16x2(acc[2 * i], acc[2 * i + 1]);
+                    for (int i = 0; i < 4; ++i)
+                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(tile + lane * PITCH + k * 64 + i * 16), "f"(acc[4 * i]), "f"(acc[4 * i + 1]), "f"(acc[4 * i + 2]), "f"(acc[4 * i + 3]) : "memory");
+                } else {
+                    uint32_t o[GROUP / 2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + lane * PITCH + k * 32 + i * 16), "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3]) : "memory");
+                    for (int i = 0; i < GROUP / 2; ++i) o[i] = pack_bf16x2(acc[2 * i], acc[2 * i + 1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + lane * PITCH + k * 32 + i * 16), "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3]) : "memory");
+                }
             }
             const int per_row = 2 * my_count, magic = (65536 + per_row - 1) / per_row;  // 16-byte pieces of a row (exact for the 256 there are at most)
             const int end = min(32, rows - (warp & 3) * 32);
@@ -1089,8 +1115,20 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                 int r, c;
                 if (!place_of(k * 32 + lane, r, c)) break;
                 uint32_t v[4];
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(tile + r * PITCH + c * 16));
-                if constexpr (GATE) {
+                if constexpr (ONCE) {
+                    const uint32_t g[4] = {gate[k].x, gate[k].y, gate[k].z, gate[k].w};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float f[4];
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(tile + r * PITCH + c * 32 + i * 16));
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            v[2 * i + e] = pack_bf16x2(f[2 * e] * sigmoid(__uint_as_float(g[2 * i + e] << 16)), f[2 * e + 1] * sigmoid(__uint_as_float(g[2 * i + e] & 0xffff0000u)));
+                    }
+                } else {
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(tile + r * PITCH + c * 16));
+                }
+                if constexpr (GATE && !ONCE) {
                     const uint32_t g[4] = {gate[k].x, gate[k].y, gate[k].z, gate[k].w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i)  // bf16(attention) * sigmoid(gate): the rounding order of the two-launch form

@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
+#include <vector>
 
 #include "../../include/arc_sdpa.h"
 
@@ -43,7 +44,7 @@ const Tensor& need_tensor(PyObject* o, c10::ScalarType type, const char* name) {
     if (!t || !t->is_cuda()) bad(std::string(name) + " must be a CUDA tensor (there is no CPU path)");
     if (t->scalar_type() != type) {
         const char* want = type == at::kBFloat16 ? "torch.bfloat16" : type == at::kFloat ? "torch.float32"
-                           : type == at::kInt    ? "torch.int32"    : "torch.int64";
+                           : type == at::kInt    ? "torch.int32"    : type == at::kDouble ? "torch.float64" : "torch.int64";
         bad(std::string(name) + " must be " + want + ", got " + c10::toString(t->scalar_type()));
     }
     return *t;
@@ -61,6 +62,12 @@ int64_t to_int(PyObject* o) {  // int(o)
     Py_DECREF(n);
     if (v == -1 && PyErr_Occurred()) python_failed();
     return v;
+}
+
+int32_t to_int32(PyObject* o, const char* name) {
+    const int64_t v = to_int(o);
+    if (v != (int32_t)v) bad(std::string(name) + " does not fit 32 bits");
+    return (int32_t)v;
 }
 
 float to_float(PyObject* o) {
@@ -230,6 +237,7 @@ struct PrefillExtra {
     PyObject* workspace = nullptr;
     float* lse = nullptr;
     int num_splits = 0;
+    int sinks = 0;
 };
 
 // The one prefill call.  q, k, v, out (and gate) are four-dimensional views on `device`.
@@ -260,6 +268,7 @@ void run_prefill(c10::Device device, const View& q, const View& k, const View& v
     token_strides(out, "out", &p.o_stride_b, &p.o_stride_t);
     need_room(out, B, S, q.n[2] * q.n[3], "out");
     p.scale = scale, p.mask_type = mask_type, p.window = (int32_t)window, p.num_splits = x.num_splits;
+    p.sinks = x.sinks;
     if (!is_none(x.block_ids)) {
         const Tensor& ids = need_tensor(x.block_ids, at::kInt, "block_ids");
         if (!ids.is_contiguous() || ids.numel() < x.block_ids_offset + L || x.block_ids_offset < 0)
@@ -293,10 +302,10 @@ PyObject* again(PyObject* o) {
 }
 
 // sdpa_prefill(q, k, v, scale, mask_type, window, mask, gate, out, num_splits, return_lse, workspace, block_ids,
-//              block_ids_offset, out_copies)
+//              block_ids_offset, out_copies, sinks)
 PyObject* py_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    need_args(n, 15, "sdpa_prefill");
+    need_args(n, 16, "sdpa_prefill");
     const Tensor& tq = need_tensor(a[0], at::kBFloat16, "q");
     const Tensor& tk = need_tensor(a[1], at::kBFloat16, "k");
     const Tensor& tv = need_tensor(a[2], at::kBFloat16, "v");
@@ -334,6 +343,7 @@ PyObject* py_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x.mask = a[6], x.workspace = a[11], x.block_ids = a[12], x.out_copies = a[14];
     x.num_splits = (int)to_int(a[9]);
     x.block_ids_offset = to_int(a[13]);
+    x.sinks = to_int32(a[15], "sinks");
     run_prefill(tq.device(), q, k, v, out, to_float(a[3]), (int)to_int(a[4]), to_int(a[5]), x);
     PyObject* res = made.defined() ? wrap(made) : again(a[8]);
     if (!want_lse) return res;
@@ -656,6 +666,257 @@ PyObject* py_qkv_prepare(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// --------------------------------------------------------------------------- paged cache
+void same_device(const Tensor& t, const Tensor& ref, const char* name) {
+    if (t.device() != ref.device()) bad(std::string(name) + " is on another device than the rest of the call");
+}
+
+// A contiguous one-dimensional tensor of at least n values (exactly: of n), on ref's device; its address.
+template <typename T>
+T* vector_of(PyObject* o, c10::ScalarType type, int64_t n, bool exactly, const Tensor& ref, const char* name) {
+    const Tensor& t = need_tensor(o, type, name);
+    same_device(t, ref, name);
+    if (t.dim() != 1 || !t.is_contiguous() || (exactly ? t.size(0) != n : t.size(0) < n))
+        bad(std::string(name) + " must be contiguous, one-dimensional and hold " + std::to_string(n) + " values");
+    return static_cast<T*>(t.data_ptr());
+}
+
+// (batch, width) int32 rows
+const Tensor& table_of(PyObject* o, const Tensor& ref, int64_t batch) {
+    const Tensor& t = need_tensor(o, at::kInt, "block_table");
+    same_device(t, ref, "block_table");
+    if (t.dim() != 2 || t.size(0) != batch || t.size(1) < 1 || t.stride(1) != 1 || (batch > 1 && t.stride(0) < t.size(1)))
+        bad("block_table must be (batch, width) int32 with contiguous rows that do not overlap");
+    return t;
+}
+
+// (num_pages, page_size, nkv, hd)
+View pool_of(PyObject* o, const Tensor& ref, int64_t nkv, int64_t hd, const char* name) {
+    const Tensor& t = need_tensor(o, at::kBFloat16, name);
+    same_device(t, ref, name);
+    const View v = view_of(t, name);
+    if (v.dim != 4 || v.n[2] != nkv || v.n[3] != hd) bad(std::string(name) + " must be (num_pages, page_size, nkv, head_dim)");
+    if (v.st[3] != 1 || v.st[2] != hd) bad(std::string(name) + ": the (heads, head_dim) block of every row must be contiguous");
+    if (v.n[0] > 0x7fffffffll || v.n[1] > 0x7fffffffll) bad(std::string(name) + " is too large");
+    return v;
+}
+
+// (tokens, heads, hd) rows
+View rows_of(PyObject* o, const Tensor& ref, int64_t tokens, int64_t heads, int64_t hd, const char* name) {
+    const Tensor& t = need_tensor(o, at::kBFloat16, name);
+    same_device(t, ref, name);
+    const View v = view_of(t, name);
+    if (v.dim != 3 || v.n[0] != tokens || (heads >= 0 && v.n[1] != heads) || v.n[2] != hd)
+        bad(std::string(name) + " must be (tokens, heads, head_dim), as the rest of the call");
+    if (v.st[2] != 1 || v.st[1] != hd) bad(std::string(name) + ": the (heads, head_dim) block of every token must be contiguous");
+    return v;
+}
+
+// Bytes [lo, hi) of a tensor's elements.
+void extent_of(const Tensor& t, uintptr_t* lo, uintptr_t* hi) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    *lo = reinterpret_cast<uintptr_t>(t.data_ptr());
+    *hi = t.numel() ? *lo + (uintptr_t)(last + 1) * t.element_size() : *lo;
+}
+
+bool overlap(const Tensor& a, const Tensor& b) {
+    uintptr_t a0, a1, b0, b1;
+    extent_of(a, &a0, &a1);
+    extent_of(b, &b0, &b1);
+    return a0 < b1 && b0 < a1;
+}
+
+// paged_tables(new_len, past_len, block_table, free_pages, free_begin, page_size, num_tokens, out)
+//   -> (slots, positions, token_begin, kv_len, pages_used)
+PyObject* py_paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    need_args(n, 8, "paged_tables");
+    const Tensor& ref = need_tensor(a[0], at::kInt, "new_len");
+    if (ref.dim() != 1) bad("new_len must be one-dimensional");
+    const int64_t B = ref.size(0);
+    arc_paged_tables_params p{};
+    p.new_len = vector_of<int32_t>(a[0], at::kInt, B, true, ref, "new_len");
+    if (!is_none(a[1])) p.past_len = vector_of<int32_t>(a[1], at::kInt, B, true, ref, "past_len");
+    const Tensor& table = table_of(a[2], ref, B);
+    p.block_table = static_cast<int32_t*>(table.data_ptr());
+    if (B > 0x7fffffffll || table.size(1) > 0x7fffffffll) bad("block_table is too large");
+    p.batch = (int32_t)B, p.table_width = (int32_t)table.size(1), p.table_stride = B > 1 ? table.stride(0) : table.size(1);
+    const Tensor& list = need_tensor(a[3], at::kInt, "free_pages");
+    p.free_pages = vector_of<int32_t>(a[3], at::kInt, 0, false, ref, "free_pages");
+    if (list.size(0) > 0x7fffffffll) bad("free_pages is too large");
+    p.free_count = (int32_t)list.size(0);
+    if (!is_none(a[4])) p.free_begin = vector_of<int32_t>(a[4], at::kInt, 1, true, ref, "free_begin");
+    p.page_size = to_int32(a[5], "page_size"), p.num_tokens = to_int32(a[6], "num_tokens");
+    if (p.num_tokens < 0) bad("num_tokens must not be negative");
+    const char* names[5] = {"slots", "positions", "token_begin", "kv_len", "pages_used"};
+    const int64_t sizes[5] = {p.num_tokens, p.num_tokens, B + 1, B, 1};
+    const Held made(is_none(a[7]) ? PyTuple_New(5) : nullptr);
+    int32_t* to[5];
+    if (made.o) {
+        // One allocation (five took 4 us of host time)
+        Tensor all = new_cuda({2 * sizes[0] + sizes[2] + sizes[3] + 1}, at::kInt, ref.device());
+        const std::vector<Tensor> parts = all.split_with_sizes(at::IntArrayRef(sizes, 5));
+        for (int i = 0; i < 5; ++i) {
+            to[i] = static_cast<int32_t*>(parts[i].data_ptr());
+            PyTuple_SET_ITEM(made.o, i, wrap(parts[i]));
+        }
+    } else {
+        if (!PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 5) bad("out must be a tuple (slots, positions, token_begin, kv_len, pages_used)");
+        for (int i = 0; i < 5; ++i) {
+            to[i] = vector_of<int32_t>(PyTuple_GET_ITEM(a[7], i), at::kInt, sizes[i], true, ref, names[i]);
+            const Tensor& t = *tensor_or_null(PyTuple_GET_ITEM(a[7], i));
+            bool twice = overlap(t, table) || overlap(t, ref) || overlap(t, list);
+            for (int k : {1, 4}) twice |= !is_none(a[k]) && overlap(t, *tensor_or_null(a[k]));
+            for (int k = 0; k < i; ++k) twice |= overlap(t, *tensor_or_null(PyTuple_GET_ITEM(a[7], k)));
+            if (twice) bad(std::string(names[i]) + " overlaps another tensor of the call");
+        }
+    }
+    p.slots = to[0], p.positions = to[1], p.token_begin = to[2], p.kv_len = to[3], p.pages_used = to[4];
+    const c10::cuda::CUDAGuard guard(ref.device());
+    void* stream = c10::cuda::getCurrentCUDAStream(ref.device().index()).stream();
+    check_status(without_gil([&] { return arc_paged_tables(&p, stream); }), "arc_paged_tables");
+    return again(made.o ? made.o : a[7]);
+    END_HANDLE_TH_ERRORS
+}
+
+// qkv_prepare_paged(q, k, v, positions, inv_freq, k_pages, v_pages, slots, norm, v_norm, q_weight, k_weight, eps, interleaved,
+//                   mscale, q_out, k_out, v_out)
+PyObject* py_qkv_prepare_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    need_args(n, 18, "qkv_prepare_paged");
+    if (is_none(a[0]) && is_none(a[1])) bad("qkv_prepare_paged needs q or k");
+    const Tensor& ref = need_tensor(is_none(a[0]) ? a[1] : a[0], at::kBFloat16, is_none(a[0]) ? "k" : "q");
+    if (ref.dim() != 3) bad("q, k and v must be (tokens, heads, head_dim)");
+    const int64_t T = ref.size(0), hd = ref.size(2);
+    if (T > 0x7fffffffll) bad("too many tokens");
+    arc_qkv_prepare_paged_params p{};
+    p.tokens = (int32_t)T, p.hd = (int32_t)hd;
+    auto rows = [&](int i, int64_t heads, const char* name) { return is_none(a[i]) ? View() : rows_of(a[i], ref, T, heads, hd, name); };
+    const View q = rows(0, -1, "q"), k = rows(1, -1, "k"), v = rows(2, k.given() ? k.n[1] : -1, "v");
+    if (v.given() && !k.given()) bad("v needs k");
+    if (q.given()) {
+        const View o = is_none(a[15]) ? q : rows(15, q.n[1], "q_out");
+        p.q = q.ptr, p.q_out = o.ptr, p.nq = (int32_t)q.n[1], p.q_stride = q.st[0], p.q_out_stride = o.st[0];
+    }
+    if (k.given()) {
+        const bool paged = !is_none(a[5]);
+        if (paged != !is_none(a[6]) && v.given()) bad("k_pages and v_pages go together");
+        if (!v.given() && !is_none(a[6])) bad("v_pages needs v");
+        const View ko = is_none(a[16]) ? (paged ? View() : k) : rows(16, k.n[1], "k_out");
+        p.k = k.ptr, p.k_out = ko.ptr, p.nkv = (int32_t)k.n[1], p.k_stride = k.st[0], p.k_out_stride = ko.st[0];
+        if (v.given()) {
+            const View vo = is_none(a[17]) ? (paged ? View() : v) : rows(17, k.n[1], "v_out");
+            p.v = v.ptr, p.v_out = vo.ptr, p.v_stride = v.st[0], p.v_out_stride = vo.st[0];
+        }
+        if (paged) {
+            const View kp = pool_of(a[5], ref, k.n[1], hd, "k_pages");
+            p.k_pages = kp.ptr, p.k_stride_page = kp.st[0], p.k_stride_t = kp.st[1];
+            p.num_pages = (int32_t)kp.n[0], p.page_size = (int32_t)kp.n[1];
+            if (v.given()) {
+                const View vp = pool_of(a[6], ref, k.n[1], hd, "v_pages");
+                if (vp.n[0] != kp.n[0] || vp.n[1] != kp.n[1]) bad("k_pages and v_pages must have the same number and size of pages");
+                p.v_pages = vp.ptr, p.v_stride_page = vp.st[0], p.v_stride_t = vp.st[1];
+            }
+            if (is_none(a[7])) bad("pages need slots");
+            p.slots = vector_of<int32_t>(a[7], at::kInt, T, true, ref, "slots");
+        }
+    } else if (!is_none(a[5]) || !is_none(a[6])) {
+        bad("k_pages and v_pages need k and v");
+    }
+    p.positions = vector_of<int32_t>(a[3], at::kInt, T, true, ref, "positions");
+    if (!is_none(a[4])) {
+        const Tensor& f = need_tensor(a[4], at::kDouble, "inv_freq");
+        if (f.dim() != 1 || f.size(0) > hd / 2) bad("inv_freq must be one-dimensional, with at most head_dim / 2 values");
+        p.inv_freq = vector_of<double>(a[4], at::kDouble, f.size(0), true, ref, "inv_freq");
+        p.rotary_dim = (int32_t)(2 * f.size(0));
+    }
+    p.norm_qk = to_bool(a[8]), p.norm_v = to_bool(a[9]);
+    if (!p.norm_qk && (!is_none(a[10]) || !is_none(a[11]))) bad("weights need norm=True");
+    if (!is_none(a[10])) p.q_weight = vector_of<void>(a[10], at::kBFloat16, hd, true, ref, "q_weight");
+    if (!is_none(a[11])) p.k_weight = vector_of<void>(a[11], at::kBFloat16, hd, true, ref, "k_weight");
+    p.eps = to_float(a[12]), p.interleaved = to_bool(a[13]), p.mscale = to_float(a[14]);
+    const c10::cuda::CUDAGuard guard(ref.device());
+    void* stream = c10::cuda::getCurrentCUDAStream(ref.device().index()).stream();
+    check_status(without_gil([&] { return arc_qkv_prepare_paged(&p, stream); }), "arc_qkv_prepare_paged");
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// sdpa_decode_paged(q, k_pages, v_pages, block_table, kv_len, scale, window, sinks, gate, out, return_partial, want_out, num_ctas,
+//                   partial_out, partial_lse, workspace)
+PyObject* py_decode_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    need_args(n, 16, "sdpa_decode_paged");
+    const Tensor& tq = need_tensor(a[0], at::kBFloat16, "q");
+    const View q = view_of(tq, "q");
+    if (q.dim != 3) bad("q must be (B, nq, hd)");
+    const int64_t B = q.n[0], nq = q.n[1], hd = q.n[2];
+    if (q.st[2] != 1 || q.st[1] != hd) bad("q: (nq, hd) must be contiguous");
+    const Tensor& tk = need_tensor(a[1], at::kBFloat16, "k_pages");
+    if (tk.dim() != 4) bad("k_pages must be (num_pages, page_size, nkv, head_dim)");
+    const View k = pool_of(a[1], tq, tk.size(2), hd, "k_pages"), v = pool_of(a[2], tq, tk.size(2), hd, "v_pages");
+    if (v.n[0] != k.n[0] || v.n[1] != k.n[1]) bad("k_pages and v_pages must have the same number and size of pages");
+    const Tensor& table = table_of(a[3], tq, B);
+    if (B > 0x7fffffffll || table.size(1) > 0x7fffffffll) bad("block_table is too large");
+    arc_sdpa_decode_paged_params p{};
+    p.q = q.ptr, p.k_pages = k.ptr, p.v_pages = v.ptr;
+    p.batch = (int32_t)B, p.nq = (int32_t)nq, p.nkv = (int32_t)k.n[2], p.hd = (int32_t)hd;
+    p.num_pages = (int32_t)k.n[0], p.page_size = (int32_t)k.n[1];
+    p.k_stride_page = k.st[0], p.k_stride_t = k.st[1], p.v_stride_page = v.st[0], p.v_stride_t = v.st[1];
+    p.q_stride_b = q.st[0];
+    p.block_table = static_cast<const int32_t*>(table.data_ptr());
+    p.table_width = (int32_t)table.size(1), p.table_stride = B > 1 ? table.stride(0) : table.size(1);
+    if (tensor_or_null(a[4])) p.kv_len = vector_of<int32_t>(a[4], at::kInt, B, true, tq, "kv_len");
+    else p.kv_len_uniform = to_int32(a[4], "kv_len");
+    p.scale = to_float(a[5]), p.window = to_int32(a[6], "window"), p.sinks = to_int32(a[7], "sinks"), p.num_ctas = to_int32(a[12], "num_ctas");
+    Tensor made;
+    View out;
+    if (!is_none(a[9])) {
+        const Tensor& t = need_tensor(a[9], at::kBFloat16, "out");
+        same_device(t, tq, "out");
+        out = view_of(t, "out");
+    } else if (to_bool(a[11])) {
+        made = new_cuda({B, nq, hd}, at::kBFloat16, tq.device());
+        out = view_of(made, "out");
+    }
+    if (out.given()) {
+        if (out.dim != 3 || out.n[0] != B || out.n[1] != nq || out.n[2] != hd || out.st[2] != 1 || out.st[1] != hd)
+            bad("out must be laid out like q");
+        p.out = out.ptr, p.o_stride_b = out.st[0];
+    }
+    if (!is_none(a[8])) {
+        const Tensor& t = need_tensor(a[8], at::kBFloat16, "gate");
+        same_device(t, tq, "gate");
+        const View gate = view_of(t, "gate");
+        if (!out.given() || !same_layout(gate, out)) bad("gate must be laid out like out");
+        p.gate = gate.ptr;
+    }
+    const bool partial = to_bool(a[10]);
+    Tensor o32, lse;
+    if (partial) {
+        o32 = is_none(a[13]) ? new_cuda({B, nq, hd}, at::kFloat, tq.device()) : need_tensor(a[13], at::kFloat, "partial_out");
+        lse = is_none(a[14]) ? new_cuda({B, nq}, at::kFloat, tq.device()) : need_tensor(a[14], at::kFloat, "partial_lse");
+        same_device(o32, tq, "partial_out");
+        same_device(lse, tq, "partial_lse");
+        const bool shapes = o32.dim() == 3 && o32.size(0) == B && o32.size(1) == nq && o32.size(2) == hd && lse.dim() == 2 && lse.size(0) == B && lse.size(1) == nq;
+        if (!shapes || !o32.is_contiguous() || !lse.is_contiguous())
+            bad("partial_out / partial_lse must be contiguous (B, nq, hd) / (B, nq) f32");
+        p.out_f32 = static_cast<float*>(o32.data_ptr());
+        p.out_lse = static_cast<float*>(lse.data_ptr());
+    }
+    const c10::cuda::CUDAGuard guard(tq.device());
+    const size_t need = arc_sdpa_decode_paged_workspace_bytes(&p);
+    Scratch scratch;
+    if (need) scratch.take(a[15], need, &p.workspace, &p.workspace_bytes);
+    void* stream = c10::cuda::getCurrentCUDAStream(tq.device().index()).stream();
+    check_status(without_gil([&] { return arc_sdpa_decode_paged(&p, stream); }), "arc_sdpa_decode_paged");
+    PyObject* res = made.defined() ? wrap(made) : again(is_none(a[9]) ? Py_None : a[9]);
+    if (!partial) return res;
+    return Py_BuildValue("(NNN)", res, wrap(o32), wrap(lse));
+    END_HANDLE_TH_ERRORS
+}
+
 // --------------------------------------------------------------------------- small calls
 // mul_sigmoid_inplace(a, gate) -> a
 PyObject* py_mul_sigmoid(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -708,6 +969,9 @@ PyMethodDef g_methods[] = {
     ARC_METHOD("decode_one", py_decode_one),
     ARC_METHOD("qwen_attention", py_qwen_attention),
     ARC_METHOD("qkv_prepare", py_qkv_prepare),
+    ARC_METHOD("paged_tables", py_paged_tables),
+    ARC_METHOD("qkv_prepare_paged", py_qkv_prepare_paged),
+    ARC_METHOD("sdpa_decode_paged", py_decode_paged),
     ARC_METHOD("mul_sigmoid_inplace", py_mul_sigmoid),
     ARC_METHOD("fill_causal_mask", py_fill_causal_mask),
     {nullptr, nullptr, 0, nullptr},

@@ -8,6 +8,7 @@ map one to one (reference files are cited per function).
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional, Union
 
 import torch
@@ -20,6 +21,7 @@ __all__ = [
     "sdpa_prefill", "sdpa_decode", "sdpa_merge", "mul_sigmoid_inplace", "fill_causal_mask",
     "gqa_attention_sdpa", "gqa_attention", "batched_attention", "qwen35_xmx_attention",
     "qwen35_online_attention", "qwen35_xmx_attention_decode_gqa",
+    "paged_tables", "rope_frequencies", "qkv_prepare_paged", "sdpa_decode_paged",
     "device_status", "clear_device_status", "launch_count", "Workspace", "exchange_bytes",
 ]
 
@@ -80,7 +82,7 @@ def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: fl
                  num_splits: int = 0, return_lse: bool = False,
                  workspace: Optional[Workspace] = None,
                  block_ids: Optional[torch.Tensor] = None, block_ids_offset: int = 0,
-                 out_copies: Optional[torch.Tensor] = None):
+                 out_copies: Optional[torch.Tensor] = None, sinks: int = 0):
     """Prefill / canvas attention.  q: (B, S, nq, hd) or (S, nq, hd); k, v: (B, L, nkv, hd) or (L, nkv, hd).
 
     ``out`` may be ``q`` itself.  Returns ``out`` (and the natural-log LSE (B, S, nq) when asked).
@@ -90,9 +92,12 @@ def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: fl
     ``out_copies`` (device int64, at most 15 addresses): further buffers laid out like ``out`` that the
     kernel's epilogue stores the result to as well — other GPUs' mapped buffers when a head-sharded output
     is to be gathered (see ``sharded.GatheredPrefill``).
+    ``sinks`` (causal masks without block ids): the first keys stay visible behind the window, too — the query at
+    position i sees keys j <= i with j < sinks or j > i - window.  With ``sinks`` > 0 a gated result is rounded once, after
+    the gate (otherwise also before it, as the reference does).
     """
     return _native().sdpa_prefill(q, k, v, scale, mask_type, window, mask, gate, out, num_splits, return_lse, workspace,
-                                  block_ids, block_ids_offset, out_copies)
+                                  block_ids, block_ids_offset, out_copies, sinks)
 
 
 def sdpa_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float,
@@ -324,6 +329,107 @@ def fused_norm_rope_inplace(x: torch.Tensor, weight: torch.Tensor, offset: int, 
     qkv_prepare(x, None, None, q_weight=weight, eps=eps, theta=theta, partial_rotary_factor=partial,
                 rope_cos=rope_cos, rope_sin=rope_sin, pos_offset=offset)
     return x
+
+
+# ---------------------------------------------------------------------------
+# Paged KV cache: pools of pages (num_pages, page_size, nkv, hd), a block table row per request
+# ---------------------------------------------------------------------------
+def paged_tables(new_len: torch.Tensor, past_len: Optional[torch.Tensor], block_table: torch.Tensor, free_pages: torch.Tensor, *,
+                 page_size: int, num_tokens: int, free_begin: Optional[torch.Tensor] = None, out: Optional[tuple] = None):
+    """Block tables and slot maps of one step, built on the device from the requests' lengths: one launch, nothing copied to the host.
+
+    ``new_len``, ``past_len`` (B,) int32: tokens that each request adds (0: none) and has in the cache (None: none).
+    ``block_table`` (B, width) int32: rows hold the pages of the past tokens; the pages that the new ones need besides
+    come from ``free_pages`` (int32, from entry ``free_begin[0]`` on), requests in order, and are written behind them.
+    ``num_tokens``: room for the step's tokens, at least their sum.  B <= 2048; ``page_size`` a multiple of 16.
+
+    Returns ``(slots, positions, token_begin, kv_len, pages_used)``, int32, or writes them to the tuple ``out``:
+    ``slots`` (num_tokens,) = page * page_size + row of every token and ``positions`` its place in its request, requests
+    packed in order, -1 behind the last token; ``token_begin`` (B + 1,); ``kv_len`` (B,) = past + new; ``pages_used`` (1,)
+    = pages the step needs from the list.  If that is more than the list holds, entries and slots without a page are -1.
+    A length that is negative or does not fit its row, or more than ``num_tokens`` tokens, shows in ``device_status()``
+    (``FAULT_BAD_KV_RANGE``; detail: the request, B for the sum), and nothing is written.
+    """
+    return _native().paged_tables(new_len, past_len, block_table, free_pages, free_begin, page_size, num_tokens, out)
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
+                     original_len: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0, device="cuda"):
+    """``(inv_freq, mscale)`` for :func:`qkv_prepare_paged`: radians per position of every pair, float64 (rotary_dim / 2,), and
+    the factor on cosine and sine.
+
+    ``scaling``, for contexts ``factor`` times as long as ``original_len``, which the model was trained on: None; ``"linear"``
+    (positions divided by the factor); ``"ntk"`` (theta times factor^(d / (d - 2)): the slowest pair turns ``factor`` times
+    slower, the fastest as before); ``"yarn"`` (arXiv:2309.00071: pairs that turn less than ``beta_slow`` times over
+    ``original_len`` are divided by the factor, those over ``beta_fast`` times are left, a ramp between; mscale =
+    0.1 ln(factor) + 1)."""
+    if rotary_dim <= 0 or rotary_dim % 16 != 0:
+        raise ValueError("rotary_dim must be a positive multiple of 16")
+    if not theta > 0.0 or not math.isfinite(theta):
+        raise ValueError("theta must be positive")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError("scaling must be None, 'linear', 'ntk' or 'yarn'")
+    if scaling is not None and not (factor >= 1.0 and math.isfinite(factor)):
+        raise ValueError("factor must be at least 1")
+    base = theta * factor ** (rotary_dim / (rotary_dim - 2)) if scaling == "ntk" else theta
+    inv = [base ** (-2.0 * f / rotary_dim) for f in range(rotary_dim // 2)]
+    mscale = 1.0
+    if scaling == "linear":
+        inv = [w / factor for w in inv]
+    if scaling == "yarn":
+        if original_len <= 0 or not beta_fast > beta_slow:
+            raise ValueError("yarn needs original_len and beta_fast > beta_slow")
+
+        def kept(w):
+            return min(1.0, max(0.0, (original_len * w / (2 * math.pi) - beta_slow) / (beta_fast - beta_slow)))
+
+        inv = [w * kept(w) + w / factor * (1.0 - kept(w)) for w in inv]
+        mscale = 0.1 * math.log(factor) + 1.0
+    return torch.tensor(inv, dtype=torch.float64, device=device), mscale
+
+
+def qkv_prepare_paged(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Optional[torch.Tensor], positions: torch.Tensor,
+                      inv_freq: Optional[torch.Tensor], *, k_pages: Optional[torch.Tensor] = None,
+                      v_pages: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None, norm: bool = True,
+                      v_norm: bool = False, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                      eps: float = 1e-6, interleaved: bool = False, mscale: float = 1.0, q_out: Optional[torch.Tensor] = None,
+                      k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None) -> None:
+    """:func:`qkv_prepare` for packed tokens and a paged cache: RMSNorm of the projected Q / K rows per head, rotation and
+    append, one launch.
+
+    q (T, nq, hd), k, v (T, nkv, hd); ``positions`` (T,) int32; ``inv_freq`` float64 (rotary_dim / 2,) on the device and ``mscale`` as
+    :func:`rope_frequencies` gives them (None: no rotation).  Pairs are (f, f + rotary_dim / 2), or (2 f, 2 f + 1) with
+    ``interleaved``; rotary_dim a multiple of 16, the rest of the head is not rotated.  Angles are exact at any position.
+    Norm and rotation are in fp32 and rounded once (:func:`qkv_prepare` rounds between them, as the reference does).
+    ``norm=False`` rotates only; ``v_norm`` gives V rows a unit-RMS norm.
+
+    Q is rewritten in place or goes to ``q_out``.  K and V go to rows ``slots`` (T,) of ``k_pages`` / ``v_pages`` (num_pages,
+    page_size, nkv, hd), and to ``k_out`` / ``v_out`` if given (which may be k and v: a prompt's attention reads them there);
+    without pages they are rewritten in place.  A slot of -1 is not appended; a token with a negative position is padding,
+    of which nothing is read or written.  Slots of a call must differ; one outside the pool is not written and shows in
+    ``device_status()`` (``FAULT_BAD_KV_RANGE``; detail: the token).
+    """
+    _native().qkv_prepare_paged(q, k, v, positions, inv_freq, k_pages, v_pages, slots, norm, v_norm, q_weight, k_weight, eps,
+                                interleaved, mscale, q_out, k_out, v_out)
+
+
+def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                      kv_len: Union[int, torch.Tensor], *, scale: float, window: int = NO_WINDOW, sinks: int = 0,
+                      gate: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, return_partial: bool = False,
+                      want_out: bool = True, num_ctas: int = 0, partial_out: Optional[torch.Tensor] = None,
+                      partial_lse: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None):
+    """:func:`sdpa_decode` over a paged cache: one query token per sequence, split over the keys and joined.
+
+    q (B, nq, hd); ``k_pages``, ``v_pages`` (num_pages, page_size, nkv, hd); ``block_table`` (B, width) int32: token t of sequence b
+    is row t % page_size of page ``block_table[b, t // page_size]``; ``kv_len``: int or int32 device tensor (B,), the token
+    itself included.  ``window``: the last keys that are seen; ``sinks``: the first ones that stay visible behind it.  Pages
+    without such a key are not looked at (their entries may be anything).  A sequence without keys gives zeros, lse -inf.
+    Returns ``out`` (B, nq, hd) bf16, rounded once, after the gate; with ``return_partial`` also (out_f32, lse), ungated.
+    A length beyond its table row, or an entry outside the pool, shows in ``device_status()`` (``FAULT_BAD_KV_RANGE``; detail:
+    the sequence), and the outputs are left unwritten.
+    """
+    return _native().sdpa_decode_paged(q, k_pages, v_pages, block_table, kv_len, scale, window, sinks, gate, out, return_partial,
+                                       want_out, num_ctas, partial_out, partial_lse, workspace)
 
 
 def exchange_bytes(world: int, batch: int, nq: int, hd: int) -> int:

@@ -34,7 +34,7 @@ extern "C" {
 #define ARC_OK 0
 #define ARC_ERR_BAD_SHAPE 1            /* non-positive size, nq % nkv != 0, ... */
 #define ARC_ERR_ALIGNMENT 2            /* pointer or stride not 16-byte aligned */
-#define ARC_ERR_UNSUPPORTED_HEAD_DIM 3 /* hd not in {128, 256} (attention) / {128, 256, 512} (qkv_prepare) */
+#define ARC_ERR_UNSUPPORTED_HEAD_DIM 3 /* hd not in {128, 256} (attention) / {128, 256, 512} (qkv_prepare, qkv_prepare_paged) */
 #define ARC_ERR_WORKSPACE_TOO_SMALL 4
 #define ARC_ERR_CUDA 5                 /* a CUDA runtime / driver call failed */
 #define ARC_ERR_COLLECTIVE 6           /* NCCL missing or a collective failed (arc_sdpa_allgather_merge) */
@@ -42,7 +42,7 @@ extern "C" {
 #define ARC_ERR_NULL_POINTER 8
 #define ARC_ERR_UNSUPPORTED_GQA 9      /* decode: more than 16 query heads per KV head */
 #define ARC_ERR_TOO_LARGE 10           /* size beyond a documented fixed limit */
-#define ARC_ERR_DEVICE_BAD_RANGE 11    /* a device-side kv_len / kv_row_offset reaches past the cache (see
+#define ARC_ERR_DEVICE_BAD_RANGE 11    /* a device-side length, row offset, page or slot reaches past the cache (see
                                           arc_sdpa_device_status) */
 
 /* ---- mask types: the values the reference hands to oneDNN's sdpa
@@ -115,6 +115,10 @@ typedef struct arc_sdpa_prefill_params {
      * caller's business (a barrier, a flag).  Entries must be 16-byte aligned; lse is not copied. */
     const uint64_t* out_copies;
     int32_t out_copy_count;
+    /* The first `sinks` keys stay visible behind a window (optional, ARC_MASK_CAUSAL without block_ids): query at
+     * position i sees keys j <= i with j < sinks or j > i - window.  0: none; without a window they change nothing.
+     * With sinks > 0 a gated result is rounded once, after the gate, and out_lse is that of the sums before any rounding. */
+    int32_t sinks;
 } arc_sdpa_prefill_params;
 
 size_t arc_sdpa_prefill_workspace_bytes(const arc_sdpa_prefill_params* p);
@@ -304,6 +308,112 @@ typedef struct arc_qkv_prepare_params {
 } arc_qkv_prepare_params;
 
 int arc_qkv_prepare(const arc_qkv_prepare_params* p, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Serving from a paged KV cache.  No counterpart in the reference, whose caches are one block per layer
+ * (src/modeling/qwen3_5/cache.hpp:9-14).  K and V of a layer are pools of `num_pages` pages of `page_size` rows of
+ * (nkv, hd); a row of the block table lists a request's pages in order, so its token t is row t % page_size of page
+ * table[t / page_size]; a slot is page * page_size + row.  page_size: a multiple of 16.  One table serves all layers.
+ *
+ * A step of a batch: arc_paged_tables (once), then per layer arc_qkv_prepare_paged and arc_sdpa_decode_paged (or, for a
+ * prompt, arc_sdpa_prefill over the rows that arc_qkv_prepare_paged has also left in k_out / v_out).
+ * --------------------------------------------------------------------------- */
+
+/* Block tables and slot maps of one step, on the device from the requests' lengths, one launch.
+ * Request b has past_len[b] tokens in the cache (NULL: none) and adds new_len[b] (may be 0).  Its table row must hold the pages of the
+ * past tokens; the pages its new ones need besides are taken from free_pages[free_begin ..], requests in order, and
+ * written behind them; the rest of the row is left as it was.  Token i of the step (requests in order, packed) gets
+ * positions[i], its place in its request, and slots[i]; kv_len[b] = past + new; token_begin[b] = first token of request
+ * b, token_begin[batch] their number; pages_used[0] = pages the step needs from the list.  Where the list is too short for that,
+ * table entries and slots without a page are -1.  Entries of slots / positions behind the last token, up to num_tokens,
+ * are -1 (padding that arc_qkv_prepare_paged passes over), so that a captured step may bring fewer tokens.
+ * A negative length, one that does not fit the table's row, or more than num_tokens tokens: nothing is written, and
+ * arc_sdpa_device_status() shows ARC_ERR_DEVICE_BAD_RANGE (detail: the request; batch where the sum is too large).
+ * batch <= 2048.  kv_len must not overlap past_len.  4-byte alignment is enough. */
+typedef struct arc_paged_tables_params {
+    const int32_t* new_len;    /* [batch] */
+    const int32_t* past_len;   /* [batch] or NULL */
+    int32_t* block_table;      /* (batch, table_width), rows table_stride entries apart */
+    const int32_t* free_pages; /* [free_count] */
+    const int32_t* free_begin; /* [1]: entries of free_pages that are used up already; or NULL: none */
+    int32_t* slots;            /* [num_tokens] */
+    int32_t* positions;        /* [num_tokens] */
+    int32_t* token_begin;      /* [batch + 1] */
+    int32_t* kv_len;           /* [batch] */
+    int32_t* pages_used;       /* [1] */
+    int32_t batch, num_tokens, page_size, table_width, free_count;
+    int64_t table_stride;
+} arc_paged_tables_params;
+
+int arc_paged_tables(const arc_paged_tables_params* p, void* stream);
+
+/* arc_qkv_prepare for packed tokens and a paged cache: norms of the projected Q and K rows, rotation, append, one launch.
+ * Per (token, head) row of hd values x, in fp32 and rounded once (arc_qkv_prepare rounds between norm and rotation, as
+ * the reference does):
+ *   y = x * rsqrt(mean(x^2) + eps) * weight     Q and K rows if norm_qk (weight NULL: 1), V rows if norm_v (no weight)
+ *   Q and K rows, pairs f < rotary_dim / 2:  (y[a], y[b]) = (y[a] c - y[b] s, y[a] s + y[b] c)
+ *     a, b = f, f + rotary_dim / 2 (half layout) or 2 f, 2 f + 1 (interleaved);
+ *     c, s = mscale * cos, sin(positions[token] * inv_freq[f]), the angle in 64 bits: exact however far the position.
+ * Q rows go to q_out (may be q).  K and V rows go to row slots[token] of the pages (a slot of -1: nowhere) and, if given,
+ * to k_out / v_out (may be k / v).  A token with a negative position is padding: nothing of it is read or written.
+ * A slot of num_pages * page_size or more (or below -1) is not written and shows as ARC_ERR_DEVICE_BAD_RANGE in
+ * arc_sdpa_device_status() (detail: the token).  Slots of a call must differ.  q, k and v may each be NULL; v needs k.
+ * hd in {128, 256, 512}; rotary_dim a multiple of 16, <= hd; strides in elements, multiples of 8; pointers 16-byte aligned. */
+typedef struct arc_qkv_prepare_paged_params {
+    const void* q;  /* (tokens, nq, hd) bf16, or NULL */
+    const void* k;  /* (tokens, nkv, hd) bf16, or NULL */
+    const void* v;  /* (tokens, nkv, hd) bf16, or NULL */
+    void* q_out;
+    void* k_out;    /* or NULL */
+    void* v_out;    /* or NULL */
+    void* k_pages;  /* (num_pages, page_size, nkv, hd) bf16, or NULL */
+    void* v_pages;
+    const int32_t* slots;      /* [tokens]; needed with pages */
+    const int32_t* positions;  /* [tokens] */
+    const double* inv_freq;    /* [rotary_dim / 2] radians per position; NULL with rotary_dim 0 */
+    const void* q_weight;      /* [hd] bf16 or NULL */
+    const void* k_weight;
+    int32_t tokens, nq, nkv, hd;
+    int32_t page_size, num_pages;
+    int32_t rotary_dim, interleaved, norm_qk, norm_v;
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, v_out_stride; /* elements between tokens */
+    int64_t k_stride_page, k_stride_t, v_stride_page, v_stride_t;                   /* elements between pages / rows */
+    float eps, mscale;
+} arc_qkv_prepare_paged_params;
+
+int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void* stream);
+
+/* Attention of one new token per sequence over its pages, split over the keys and joined; the paged form of
+ * arc_sdpa_decode, whose rules for out_f32 and out_lse apply; a gated result is rounded once, after the gate.  With a window the last `window` keys are seen (the
+ * token itself included) and the first `sinks`; pages that hold no such key are neither read nor looked up.  A sequence
+ * without keys gives zeros and a log-sum-exp of -inf.  A kv_len beyond table_width * page_size, or an entry outside
+ * [0, num_pages) for a page that is read, shows as ARC_ERR_DEVICE_BAD_RANGE in arc_sdpa_device_status() (detail: the
+ * sequence) and leaves the outputs unwritten.  nq / nkv <= 16, batch <= 2048, hd 128 or 256. */
+typedef struct arc_sdpa_decode_paged_params {
+    const void* q;       /* (batch, nq, hd) bf16, batch stride q_stride_b */
+    const void* k_pages; /* (num_pages, page_size, nkv, hd) bf16 */
+    const void* v_pages;
+    void* out;           /* (batch, nq, hd) bf16, batch stride o_stride_b; may be NULL */
+    const void* gate;    /* optional, laid out like out */
+    const int32_t* block_table; /* device (batch, table_width), rows table_stride entries apart */
+    const int32_t* kv_len;      /* device [batch]; NULL -> kv_len_uniform */
+    float* out_f32;      /* optional (batch, nq, hd) */
+    float* out_lse;      /* optional (batch, nq) */
+    int32_t batch, nq, nkv, hd;
+    int32_t page_size, num_pages, table_width;
+    int32_t kv_len_uniform;
+    int32_t window; /* >= 1; ARC_NO_WINDOW = off */
+    int32_t sinks;  /* >= 0 */
+    int64_t q_stride_b, o_stride_b, table_stride;
+    int64_t k_stride_page, k_stride_t, v_stride_page, v_stride_t; /* elements between pages / rows (>= nkv * hd) */
+    float scale;
+    int32_t num_ctas; /* 0 -> one per SM */
+    void* workspace;
+    size_t workspace_bytes;
+} arc_sdpa_decode_paged_params;
+
+size_t arc_sdpa_decode_paged_workspace_bytes(const arc_sdpa_decode_paged_params* p);
+int arc_sdpa_decode_paged(const arc_sdpa_decode_paged_params* p, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Multi-GPU helpers (one process per GPU).  No counterpart in the reference, whose two GPUs split
