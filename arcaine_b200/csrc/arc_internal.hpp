@@ -13,6 +13,7 @@ constexpr int kDecodeStaticSmem = 1024;
 struct HostState {
     uint32_t* fault;  // the status word kernels report to
     int sm_count, smem_optin;
+    int decode_clusters[9];  // [size]: clusters of decode CTAs the device holds at once
 };
 int host_state(HostState* out);
 

@@ -166,7 +166,67 @@ struct DecodePagedPlan {
     int nkv_cta = 1, groups = 1, slices = 1, stages = 2, ncta = 1, nt = 1, smem_bytes = 0;
     long long parts = 0;
     size_t ws_bytes = 0;
+    bool cluster = false;  // one launch: `ncta` CTAs of a cluster per sequence and group of heads
 };
+
+// Slices of 16 keys that a token at the end of `len` keys sees at most.
+static long long most_slices_seen(const arc_sdpa_decode_paged_params* p, int64_t len) {
+    if (p->window >= len) return (len + 15) / 16;
+    return std::min<long long>((len + 15) / 16, ((int64_t)p->window + 30) / 16 + ((int64_t)p->sinks + 15) / 16);
+}
+
+// Stages of 16-key slices of `heads` KV heads, `slices` each; extra: bytes behind them.  False: not even two fit.
+static bool size_paged_cta(int hd, int heads, int slices, int extra, int smem_optin, DecodePagedPlan* plan) {
+    const int stage = 64 * slices * heads * hd, fixed = 1024 + 4 * 16 + extra;
+    plan->nkv_cta = heads;
+    plan->slices = slices;
+    plan->stages = std::min(4, (smem_optin - kDecodeStaticSmem - fixed) / stage);
+    plan->smem_bytes = plan->stages * stage + fixed;
+    return plan->stages >= 2;
+}
+
+static int paged_slices(int hd, int heads) { return std::max(1, std::min(64 * 1024 / (64 * heads * hd), 8 / heads)); }
+
+// One launch or two?  Clusters take 4.8 us and the longer of two times: of a CTA of the longest sequence, which streams 65 / 70 / 85 GB/s with
+// one / two / four and more KV heads of 128 and 91 with heads of 256, and of all keys at 6.5 TB/s.  Shares read those at the same
+// rate, whatever the lengths, but cost 6.5 us and 0.03 for each sequence (the second launch, the records, shares that two
+// sequences divide).  (us, shares and clusters, all sequences as long: one token of 24/4 heads of 256 over 513 keys 7.2 and 6.2, of
+// 28/4 of 128 over 4100 11.0 and 9.8; 16 over 1028 15.5 and 11.5; 48 26.9 and 22.2; 100 43.2 and 39.2; 128 of 16/2 over 4100
+// 94 and 83.)  Lengths on the device are not known here, only what a table row can name and what a window leaves of it.  Behind a
+// window that is shorter than that, streams tend to its length; otherwise one sequence may be as long as the table says and work
+// alone in its cluster, so the form is taken where that costs at most 20 us or 1.3 times what shares do.
+static bool worth_cluster(const arc_sdpa_decode_paged_params* p, int heads, int size) {
+    const int64_t longest = p->kv_len ? (int64_t)p->table_width * p->page_size : p->kv_len_uniform;
+    const double keys = 16.0 * (double)most_slices_seen(p, longest), key = 4.0 * p->nkv * p->hd;  // bytes of one
+    const double rate = p->hd == 256 ? 91e3 : heads == 1 ? 65e3 : heads < 4 ? 70e3 : 85e3;       // bytes a us
+    const double alone = 4.8 + keys * key * heads / p->nkv / size / rate;
+    const auto shares = [&](double k) { return 6.5 + 0.03 * p->batch + k * key / 6.5e6; };
+    if (p->kv_len && p->batch > 1 && p->window >= longest) return alone <= std::max(20.0, 1.3 * shares(keys));
+    return std::max(alone, 4.8 + keys * p->batch * key / 6.5e6) <= shares(keys * p->batch);
+}
+
+static void plan_paged_cluster(const arc_sdpa_decode_paged_params* p, const HostState& hs, DecodePagedPlan* plan) {
+    if (p->num_ctas != 0 || p->batch > 1024) return;
+    // The smallest group of heads, and then the largest cluster, that are all resident at once.
+    int heads = 0, size = 0;
+    for (int c = 1; c <= plan->nkv_cta && !heads; ++c)
+        if (p->nkv % c == 0 && (long long)p->batch * (p->nkv / c) <= hs.decode_clusters[1]) heads = c;
+    for (int n = 8; heads && n >= 1 && !size; --n)
+        if ((long long)p->batch * (p->nkv / heads) <= hs.decode_clusters[n]) size = n;
+    if (!size) return;
+    if (!worth_cluster(p, heads, size)) return;
+    DecodePagedPlan one = *plan;
+    const int rows = heads * (p->nq / p->nkv);
+    int finishers = 1;
+    while (finishers * 2 <= size) finishers *= 2;
+    const int extra = 64 + 8 * ((rows + 1) & ~1) * 8 + size * rows * (p->hd / finishers) * 4 + rows * 32;
+    if (!size_paged_cta(p->hd, heads, paged_slices(p->hd, heads), extra, hs.smem_optin, &one)) return;
+    one.cluster = true;
+    one.groups = p->nkv / heads;
+    one.ncta = size;
+    one.ws_bytes = 0;
+    *plan = one;
+}
 
 static int plan_decode_paged(const arc_sdpa_decode_paged_params* p, const HostState& hs, DecodePagedPlan* plan) {
     if (!p) return ARC_ERR_NULL_POINTER;
@@ -183,17 +243,15 @@ static int plan_decode_paged(const arc_sdpa_decode_paged_params* p, const HostSt
     if (G > 16) return ARC_ERR_UNSUPPORTED_GQA;
     plan->nt = G > 8 ? 2 : 1;
     // KV heads of a CTA: the largest divisor of nkv whose rows are at most 2 KB; slices of a stage: 64 KB of K and V, eight warps.
+    int heads = 1;
     for (int c = 1; c <= p->nkv && c <= 1024 / p->hd; ++c)
-        if (p->nkv % c == 0) plan->nkv_cta = c;
-    plan->slices = std::max(1, std::min(64 * 1024 / (64 * plan->nkv_cta * p->hd), 8 / plan->nkv_cta));
-    const int stage = 64 * plan->slices * plan->nkv_cta * p->hd, fixed = 1024 + 4 * 16 + (p->batch + 2) * 8;
-    plan->stages = std::min(4, (hs.smem_optin - kDecodeStaticSmem - fixed) / stage);
-    if (plan->stages < 2) return ARC_ERR_TOO_LARGE;
-    plan->smem_bytes = plan->stages * stage + fixed;
+        if (p->nkv % c == 0) heads = c;
+    if (!size_paged_cta(p->hd, heads, paged_slices(p->hd, heads), (p->batch + 2) * 8, hs.smem_optin, plan)) return ARC_ERR_TOO_LARGE;
     plan->groups = p->nkv / plan->nkv_cta;
     plan->ncta = std::min(1024, std::max(1, p->num_ctas > 0 ? p->num_ctas : hs.sm_count / plan->groups));
     plan->parts = ((long long)plan->ncta + p->batch) * plan->slices;
     plan->ws_bytes = (size_t)plan->parts * p->nq * ((size_t)p->hd + 1) * sizeof(float);
+    plan_paged_cluster(p, hs, plan);
     return ARC_OK;
 }
 
@@ -235,6 +293,19 @@ static int launch_decode_paged(const arc_sdpa_decode_paged_params* p, const Deco
     kp.slices = plan.slices;
     kp.stages = plan.stages;
     kp.ncta = plan.ncta;
+    if (plan.cluster) {
+        kp.gate = static_cast<const uint16_t*>(p->gate);
+        kp.out = static_cast<uint16_t*>(p->out);
+        kp.out_f32 = p->out_f32;
+        kp.out_lse = p->out_lse;
+        kp.o_stride_b = p->o_stride_b;
+        const auto kernel = plan.nt == 1 ? sdpa_decode_paged_cluster_kernel<HD, 1> : sdpa_decode_paged_cluster_kernel<HD, 2>;
+        ARC_CUDA(opt_in_smem(kernel, hs.smem_optin - kDecodeStaticSmem));
+        ARC_CUDA(launch_dependent(kernel, dim3((unsigned)plan.ncta, (unsigned)plan.groups, (unsigned)p->batch), dim3(32u * (unsigned)(plan.nkv_cta * plan.slices + 1)),
+                                  (size_t)plan.smem_bytes, stream, plan.ncta, tk, tv, kp));
+        count_launch();
+        return ARC_OK;
+    }
     const auto kernel = plan.nt == 1 ? sdpa_decode_paged_kernel<HD, 1> : sdpa_decode_paged_kernel<HD, 2>;
     ARC_CUDA(opt_in_smem(kernel, hs.smem_optin - kDecodeStaticSmem));
     ARC_CUDA(launch_dependent(kernel, dim3((unsigned)plan.ncta, (unsigned)plan.groups), dim3(32u * (unsigned)(plan.nkv_cta * plan.slices + 1)),
@@ -258,10 +329,18 @@ static int launch_decode_paged(const arc_sdpa_decode_paged_params* p, const Deco
     mp.fault = hs.fault;
     mp.window = p->window;
     mp.sinks = p->sinks;
-    // 64 columns a block while that leaves at most one block per SM (arc_sdpa.cu).
-    const bool narrow = (long long)p->nq * p->batch * (HD / 64) <= hs.sm_count;
-    ARC_CUDA(launch_dependent(narrow ? sdpa_decode_merge_kernel<HD, false, 64, true> : sdpa_decode_merge_kernel<HD, false, HD, true>,
-                              dim3((unsigned)p->nq, (unsigned)p->batch, narrow ? HD / 64 : 1), dim3(MERGE_THREADS), 0, stream, 1, mp));
+    // 64 columns a block while that leaves at most one block per SM (arc_sdpa.cu); else as many rows a block as leave one for each.
+    const long long rows = (long long)p->nq * p->batch;
+    const auto blocks = [&](int n) { return (long long)(p->nq + n - 1) / n * p->batch; };
+    const auto merge = [&](auto kernel, int n) {
+        return launch_dependent(kernel, dim3((unsigned)((p->nq + n - 1) / n), (unsigned)p->batch), dim3(256), 0, stream, 1, mp);
+    };
+    if (rows * (HD / 64) <= hs.sm_count)
+        ARC_CUDA(launch_dependent(sdpa_decode_merge_kernel<HD, false, 64, true>, dim3((unsigned)p->nq, (unsigned)p->batch, HD / 64), dim3(MERGE_THREADS), 0, stream, 1, mp));
+    else if (blocks(8) >= hs.sm_count) ARC_CUDA(merge(sdpa_decode_paged_merge_kernel<HD, 8>, 8));
+    else if (blocks(4) >= hs.sm_count) ARC_CUDA(merge(sdpa_decode_paged_merge_kernel<HD, 4>, 4));
+    else if (blocks(2) >= hs.sm_count) ARC_CUDA(merge(sdpa_decode_paged_merge_kernel<HD, 2>, 2));
+    else ARC_CUDA(merge(sdpa_decode_paged_merge_kernel<HD, 1>, 1));
     count_launch();
     return ARC_OK;
 }
@@ -277,7 +356,7 @@ extern "C" int arc_sdpa_decode_paged(const arc_sdpa_decode_paged_params* p, void
     if (!p || !p->q || !p->k_pages || !p->v_pages || !p->block_table || (!p->out && !p->out_f32) || (p->gate && !p->out)) return ARC_ERR_NULL_POINTER;
     // What needs no device is refused without one.
     DecodePagedPlan plan;
-    int rc = plan_decode_paged(p, HostState{nullptr, 148, 232448}, &plan);
+    int rc = plan_decode_paged(p, HostState{nullptr, 148, 232448, {}}, &plan);
     if (rc != ARC_OK) return rc;
     if (!aligned16(p->q) || !aligned16(p->k_pages) || !aligned16(p->v_pages) || !aligned16(p->out) || !aligned16(p->gate) || !aligned16(p->out_f32) ||
         ((reinterpret_cast<uintptr_t>(p->block_table) | reinterpret_cast<uintptr_t>(p->kv_len) | reinterpret_cast<uintptr_t>(p->out_lse)) & 3u) ||
@@ -290,8 +369,8 @@ extern "C" int arc_sdpa_decode_paged(const arc_sdpa_decode_paged_params* p, void
         return rc;
     HostState hs;
     if ((rc = host_state(&hs)) != ARC_OK || (rc = plan_decode_paged(p, hs, &plan)) != ARC_OK) return rc;
-    if (!p->workspace || p->workspace_bytes < plan.ws_bytes) return ARC_ERR_WORKSPACE_TOO_SMALL;
-    if (!aligned16(p->workspace)) return ARC_ERR_ALIGNMENT;
+    if (plan.ws_bytes && (!p->workspace || p->workspace_bytes < plan.ws_bytes)) return ARC_ERR_WORKSPACE_TOO_SMALL;
+    if (plan.ws_bytes && !aligned16(p->workspace)) return ARC_ERR_ALIGNMENT;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return p->hd == 128 ? launch_decode_paged<128>(p, plan, hs, st) : launch_decode_paged<256>(p, plan, hs, st);
 }

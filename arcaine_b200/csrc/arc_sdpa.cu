@@ -13,6 +13,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <iterator>
 #include <type_traits>
 #include <mutex>
 
@@ -186,8 +187,10 @@ static int device_state(DeviceState** out) {
 int host_state(HostState* out) {
     DeviceState* ds = nullptr;
     const int rc = device_state(&ds);
-    if (rc == ARC_OK) *out = HostState{ds->fault, ds->sm_count, ds->smem_optin};
-    return rc;
+    if (rc != ARC_OK) return rc;
+    *out = HostState{ds->fault, ds->sm_count, ds->smem_optin, {}};
+    std::copy(std::begin(ds->decode_clusters), std::end(ds->decode_clusters), out->decode_clusters);
+    return ARC_OK;
 }
 
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }

@@ -29,23 +29,282 @@ struct DecodePagedParams {
     int slices;   // 16-key slices of a stage; consumer warps = nkv_cta * slices
     int stages;
     int ncta;     // grid.x
+    // One launch (sdpa_decode_paged_cluster_kernel): the results
+    const uint16_t* gate;
+    uint16_t* out;
+    float* out_f32;
+    float* out_lse;
+    long long o_stride_b;
 };
 
+// What a consumer warp holds of its KV head's group of query heads: Q^T fragments (B operand, hd x 8 heads), running maximum (log2
+// domain) and sum, O^T.
+template <int HD, int NT>
+struct GroupState {
+    uint32_t q[NT][HD / 16][2];
+    float m[NT][2], l[NT][2], o[NT][HD / 16][4];
+
+    __device__ __forceinline__ void load(const uint16_t* heads, int G) {  // heads: the group's first query head
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int n = nt * 8 + (lane >> 2);
+            const bool valid = n < G;
+            const uint16_t* src = heads + (valid ? n : 0) * HD + (lane & 3) * 2;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                q[nt][kk][0] = valid ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
+                q[nt][kk][1] = valid ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
+            }
+            m[nt][0] = m[nt][1] = -CUDART_INF_F;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
+        }
+    }
+
+    // Sum of head nt * 8 + (lane & 3) * 2 + u over the key rows.
+    __device__ __forceinline__ float sum(int nt, int u) const {
+        float ls = l[nt][u];
+        ls += __shfl_xor_sync(0xffffffffu, ls, 4);
+        ls += __shfl_xor_sync(0xffffffffu, ls, 8);
+        ls += __shfl_xor_sync(0xffffffffu, ls, 16);
+        return ls;
+    }
+};
+
+constexpr int SLICE_CHUNK = 16 * 128;  // 64 columns of a slice in shared memory: 16 rows x 128 bytes
+
+// One slice: sK, sV its head's rows in shared memory ([64-column chunk][row], 128-byte swizzle), bit k of vis: key k is seen.
+template <int HD, int NT>
+__device__ __forceinline__ void attend_slice(GroupState<HD, NT>& g, uint32_t sK, uint32_t sV, uint32_t vis, float sl) {
+    constexpr int CHUNK = SLICE_CHUNK;
+    const int lane = threadIdx.x & 31, g4 = lane >> 2;  // g4: accumulator row group
+    // Swizzled addressing: 16-byte unit u of row r sits at unit u ^ (r & 7).
+    const int key_k = lane & 15, key_v = (lane & 7) + (lane >> 4) * 8;
+    const uint32_t a_k = sK + key_k * 128, a_v = sV + key_v * 128;
+    const int xk = key_k & 7, hk = lane >> 4;
+    const int xv = key_v & 7, hv = (lane >> 3) & 1;
+    if (vis != 0xffffu) {
+        // Rows nobody sees may hold anything (never-written cache, another user's NaN): their V becomes zero, so
+        // that 0 * x stays 0; their scores are replaced below.
+        for (int u = lane; u < 16 * (HD / 8); u += 32) {
+            const int key = u / (HD / 8), c = u % (HD / 8);
+            if ((vis >> key) & 1u) continue;
+            const uint32_t a = sV + (c >> 3) * CHUNK + key * 128 + (c & 7) * 16;  // (whole rows: their units' order does not matter)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0u) : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+    }
+    // Fragments are fetched AHEAD at a time and a batch before their MMAs (decode_sm100.cuh).
+    constexpr int AHEAD = HD * NT > 256 ? 2 : 4, BATCHES = HD / 16 / AHEAD;
+    constexpr int CHAINS = NT == 1 ? 4 : 2;  // independent sums of S
+    uint32_t fr[2][AHEAD][4];
+    auto fetch_k = [&](int bt) {
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const int kk = bt * AHEAD + e;
+            ldmatrix_x4(fr[bt & 1][e], a_k + (kk >> 2) * CHUNK + ((((kk & 3) * 2 + hk) ^ xk) << 4));
+        }
+    };
+    auto fetch_v = [&](int bt) {
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const int mt = bt * AHEAD + e;
+            ldmatrix_x4_trans(fr[bt & 1][e], a_v + (mt >> 2) * CHUNK + ((((mt & 3) * 2 + hv) ^ xv) << 4));
+        }
+    };
+    float acc[NT][CHAINS][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int hh = 0; hh < CHAINS; ++hh) acc[nt][hh][0] = acc[nt][hh][1] = acc[nt][hh][2] = acc[nt][hh][3] = 0.f;
+    fetch_k(0);
+#pragma unroll
+    for (int bt = 0; bt < BATCHES; ++bt) {
+        if (bt + 1 < BATCHES) fetch_k(bt + 1);
+        else if (NT == 1) fetch_v(0);  // (an even number of batches: into the other half)
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const int kk = bt * AHEAD + e;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(acc[nt][kk % CHAINS], fr[bt & 1][e], g.q[nt][kk][0], g.q[nt][kk][1]);
+        }
+    }
+    static_assert(BATCHES % 2 == 0, "the first batch of V goes where the last one of K is not");
+    const bool v_lo = (vis >> g4) & 1u, v_hi = (vis >> (g4 + 8)) & 1u;
+    uint32_t pb[NT][2];
+    bool any_rescale = false;
+    float alpha[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float s = acc[nt][0][e] + acc[nt][1][e];
+            if constexpr (CHAINS == 4) s += acc[nt][2][e] + acc[nt][3][e];
+            s *= sl;
+            x[e] = ((e < 2) ? v_lo : v_hi) ? s : -CUDART_INF_F;
+        }
+        float pr[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float mx = fmaxf(x[u], x[u + 2]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float m_new = fmaxf(g.m[nt][u], mx);
+            const float m_eff = (m_new == -CUDART_INF_F) ? 0.f : m_new;
+            alpha[nt][u] = (m_new == -CUDART_INF_F) ? 1.f : fast_exp2(g.m[nt][u] - m_new);
+            pr[u] = fast_exp2(x[u] - m_eff);
+            pr[u + 2] = fast_exp2(x[u + 2] - m_eff);
+            g.l[nt][u] = g.l[nt][u] * alpha[nt][u] + pr[u] + pr[u + 2];
+            g.m[nt][u] = m_new;
+            any_rescale |= alpha[nt][u] != 1.f;
+        }
+        pb[nt][0] = movmatrix_trans(pack_bf16x2(pr[0], pr[1]));
+        pb[nt][1] = movmatrix_trans(pack_bf16x2(pr[2], pr[3]));
+    }
+    if (__any_sync(0xffffffffu, any_rescale)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; ++mt) {
+                g.o[nt][mt][0] *= alpha[nt][0];
+                g.o[nt][mt][1] *= alpha[nt][1];
+                g.o[nt][mt][2] *= alpha[nt][0];
+                g.o[nt][mt][3] *= alpha[nt][1];
+            }
+    }
+    if (NT > 1) fetch_v(0);
+#pragma unroll
+    for (int bt = 0; bt < BATCHES; ++bt) {
+        if (bt + 1 < BATCHES) fetch_v(bt + 1);
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(g.o[nt][bt * AHEAD + e], fr[bt & 1][e], pb[nt][0], pb[nt][1]);
+    }
+}
+
+// The ring of stages in a CTA's shared memory: [stage][K, V][slice][head][64-column chunk][row].
+struct PagedRing {
+    uint8_t* base;
+    uint64_t *full, *empty;
+    int stages, tile_bytes, slice_bytes;  // tile: K or V of a stage; slice: K or V of one
+    __device__ __forceinline__ uint8_t* slice(int stage, int v, int i) const { return base + (size_t)(2 * stage + v) * tile_bytes + i * slice_bytes; }
+};
+
+// The producer warp's side of a step of n slices; lane i has page and first row of slice i.  The stage is free.  (Whole warp, an elected lane
+// issuing: a lane per copy took 120 clk for each, and a step of eight slices of one head of 128, 16 copies, 1950 clk.)
+__device__ __forceinline__ void ask_slices(const PagedRing& r, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const DecodePagedParams& p, int st, int n, int page,
+                                           int row, int head0, int b) {
+    const int lane = threadIdx.x & 31;
+    if (lane < n && (page < 0 || page >= p.num_pages)) {
+        report_fault(p.fault, FAULT_BAD_KV_RANGE, (uint32_t)b);
+        page = p.num_pages;  // (behind the last: reads as zero)
+    }
+    if (lane == 0) mbar_arrive_expect_tx(&r.full[st], (uint32_t)(2 * n * r.slice_bytes));
+    __syncwarp();
+    for (int i = 0; i < n; ++i) {
+        const int pg = __shfl_sync(0xffffffffu, page, i), rw = __shfl_sync(0xffffffffu, row, i);
+        tma_load_5d_warp(r.slice(st, 0, i), &tm_k, &r.full[st], 0, rw, 0, head0, pg);
+        tma_load_5d_warp(r.slice(st, 1, i), &tm_v, &r.full[st], 0, rw, 0, head0, pg);
+    }
+}
+
+// Every copy issued has landed before the CTA retires (it: steps so far).
+__device__ __forceinline__ void drain(const PagedRing& r, int it) {
+    if ((threadIdx.x & 31) != 0) return;
+    for (int back = 1; back <= r.stages && back <= it; ++back) {
+        const int j = it - back;
+        mbar_wait(&r.full[j % r.stages], (j / r.stages) & 1);
+    }
+}
+
+// Folds the records of a CTA's consumer warps, of which `slices` share a KV head (hl: this warp's, slice: its place among them), through the
+// shared memory at `smem`, which nothing else uses any more.  weigh(n, s, mx, z, wt) gets maximum and sum over the slices of the KV head's
+// row n and this lane's slice's weight relative to the maximum, in eight lanes per row (s: slice, from `slices` on none), and
+// returns what the slice's values are multiplied by; store(n, d, sum) gets columns d to d + 3.  All of it runs once per call, from
+// instructions fetched cold, so loops are rolled and the weights worked out once.  (A row at a time, normalised records with
+// log-sum-exps: one token of 28/4 heads of 128 over 513 keys 9.3 us, of which the fold was 2.8.)
+template <int HD, int NT, typename W, typename S>
+__device__ __forceinline__ void fold_warps(const GroupState<HD, NT>& group, uint8_t* smem, int ncw, int nkv_cta, int slices, int hl, int slice, int G, W&& weigh, S&& store) {
+    constexpr int RS = HD + 4;  // floats from one head's row of a warp's record to the next
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, q4 = lane & 3;
+    float* rec = reinterpret_cast<float*>(smem);                                   // [warp][NT * 8 heads][RS]
+    float2* rec_ml = reinterpret_cast<float2*>(rec + (size_t)ncw * NT * 8 * RS);  // [warp][NT * 8]
+    float* rec_w = reinterpret_cast<float*>(rec_ml + ncw * NT * 8);
+    static_assert(NT * 8 * (RS + 3) <= 2 * 16 * HD, "a warp's records, sums and weights in its slices of K and V of two stages");
+    consumer_sync(ncw);  // every warp is through with the stages; no copy is in flight any more
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float ls = group.sum(nt, u);
+            const int n = warp * NT * 8 + nt * 8 + q4 * 2 + u;
+            if (g4 == 0) rec_ml[n] = make_float2(group.m[nt][u], ls);
+            float* dst = rec + (size_t)n * RS + g4;
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; ++mt) {
+                dst[mt * 16] = group.o[nt][mt][u];
+                dst[mt * 16 + 8] = group.o[nt][mt][u + 2];
+            }
+        }
+    consumer_sync(ncw);
+#pragma unroll 1
+    for (int n0 = slice * 4; n0 < G; n0 += slices * 4) {  // four rows of the KV head a turn, a lane per slice
+        const int n = n0 + (lane >> 3), s = lane & 7, at = (s * nkv_cta + hl) * NT * 8 + n;
+        const bool some = n < G && s < slices;
+        const float2 ml = some ? rec_ml[at] : make_float2(-CUDART_INF_F, 0.f);
+        float mx = ml.x;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (mx == -CUDART_INF_F) mx = 0.f;  // (nothing seen, or nothing that is a number)
+        const float wt = ml.y != ml.y ? ml.y : fast_exp2(ml.x - mx);
+        float z = ml.x == -CUDART_INF_F ? ml.y : wt * ml.y;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        const float f = weigh(n, s, mx, z, wt);
+        if (some) rec_w[at] = f;
+    }
+    consumer_sync(ncw);
+#pragma unroll 1
+    for (int i = slice; i < G * (HD / 128); i += slices) {  // half a row (head dim 256) a turn
+        const int n = i / (HD / 128), d = i % (HD / 128) * 128 + lane * 4;
+        const float* src = rec + (size_t)(hl * NT * 8 + n) * RS + d;
+        const float* wts = rec_w + hl * NT * 8 + n;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int s = 0; s < slices; ++s) {
+            const float wt = *wts;
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            acc.x = fmaf(wt, v.x, acc.x), acc.y = fmaf(wt, v.y, acc.y), acc.z = fmaf(wt, v.z, acc.z), acc.w = fmaf(wt, v.w, acc.w);
+            src += (size_t)nkv_cta * NT * 8 * RS, wts += nkv_cta * NT * 8;
+        }
+        store(n, d, acc);
+    }
+}
+
+// Equal shares: CTA x takes slices [x * per, (x + 1) * per) of all; grid.y: groups of KV heads.
 template <int HD, int NT>
 __global__ void __launch_bounds__(288, 1)
     sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                              const DecodePagedParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    constexpr int CHUNK = 16 * 128;  // 64 columns of a slice: 16 rows x 128 bytes
-    constexpr int HEAD = HD / 64 * CHUNK;
+    constexpr int HEAD = HD / 64 * SLICE_CHUNK;
 
     const int ncw = p.nkv_cta * p.slices;  // consumer warps
-    const int slice_bytes = p.nkv_cta * HEAD;  // of K or of V
-    const int tile_bytes = p.slices * slice_bytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)p.stages * 2 * tile_bytes);
-    uint64_t* empty = full + p.stages;
-    long long* cum = reinterpret_cast<long long*>(empty + p.stages);  // slices in front of each sequence
+    PagedRing ring;
+    ring.slice_bytes = p.nkv_cta * HEAD;
+    ring.tile_bytes = p.slices * ring.slice_bytes;
+    ring.base = smem;
+    ring.stages = p.stages;
+    ring.full = reinterpret_cast<uint64_t*>(smem + (size_t)p.stages * 2 * ring.tile_bytes);
+    ring.empty = ring.full + p.stages;
+    long long* cum = reinterpret_cast<long long*>(ring.empty + p.stages);  // slices in front of each sequence
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head0 = blockIdx.y * p.nkv_cta;
@@ -56,8 +315,8 @@ __global__ void __launch_bounds__(288, 1)
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], ncw);
+            mbar_init(&ring.full[s], 1);
+            mbar_init(&ring.empty[s], ncw);
         }
         fence_mbar_init();
     }
@@ -85,12 +344,10 @@ __global__ void __launch_bounds__(288, 1)
         b += n;
         if (n < 32) break;
     }
-    constexpr int RS = HD + 4;  // floats from one head's row of a warp's record to the next
-
     if (warp == ncw) {
         // ------------------------------------------------------------------ producer
-        // A step is up to `slices` slices of one sequence.  Lane i looks after K of slice i of it, lane 16 + i after V.
-        const int i = lane & 15;
+        // A step is up to `slices` slices of one sequence.
+        const int i = lane;
         struct Step {
             int n, page, row;  // slices; page and first row of this lane's slice
         };
@@ -118,278 +375,386 @@ __global__ void __launch_bounds__(288, 1)
             const int of = b;
             next = next_step();  // (its pages are on their way while this step's stage is waited for)
             const int st = it % p.stages;
-            if (it >= p.stages && !mbar_wait_warp(&empty[st], ((it / p.stages) - 1) & 1)) {
+            if (it >= p.stages && !mbar_wait_warp(&ring.empty[st], ((it / p.stages) - 1) & 1)) {
                 if (lane == 0) report_fault(p.fault, FAULT_WAIT_EMPTY, it);
                 break;
             }
-            int page = s.page;
-            if (i < s.n && (page < 0 || page >= p.num_pages)) {
-                report_fault(p.fault, FAULT_BAD_KV_RANGE, (uint32_t)of);
-                page = p.num_pages;  // (behind the last: reads as zero)
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(2 * s.n * slice_bytes));
-            __syncwarp();
-            if (i < s.n) {
-                const bool is_v = lane >= 16;
-                tma_load_5d(smem + (size_t)(2 * st + is_v) * tile_bytes + i * slice_bytes, is_v ? &tm_v : &tm_k, &full[st], 0, s.row, 0, head0, page);
-            }
-            __syncwarp();
+            ask_slices(ring, tm_k, tm_v, p, st, s.n, s.page, s.row, head0, of);
         }
-        // Every copy issued above has landed before the CTA retires.
-        if (lane == 0) {
-            for (int back = 1; back <= p.stages && back <= it; ++back) {
-                const int j = it - back;
-                mbar_wait(&full[j % p.stages], (j / p.stages) & 1);
-            }
-        }
+        drain(ring, it);
     } else if (warp < ncw) {
         // ------------------------------------------------------------------ consumers: a KV head, a slice of every step
         const int hl = warp % p.nkv_cta, slice = warp / p.nkv_cta, kvh = head0 + hl;
-        const int g4 = lane >> 2;  // accumulator row group
-        const int q4 = lane & 3;   // accumulator column pair
-        const float sl = p.scale_log2;
+        const int g4 = lane >> 2, q4 = lane & 3;  // accumulator row group, column pair
         int it = 0;
-        bool ok = true, folded = false;  // folded: this warp has been through the two barriers of the in-CTA fold
+        bool ok = true;
         long long g = g0;
+        GroupState<HD, NT> group;
         while (ok && g < g1) {
             while (cum[b + 1] <= g) ++b;
             const long long seg_end = min(g1, cum[b + 1]);
             const SeenKeys seen = seen_of(length(b), p.window, p.sinks);
             const int first = (int)(g - cum[b]), seg = (int)(seg_end - g);
-
-            // Q^T fragments (B operand, hd x 8 heads) for this head's GQA group.
-            uint32_t qf[NT][HD / 16][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int n = nt * 8 + g4;
-                const bool valid = n < G;
-                const uint16_t* qp = p.q + b * p.q_stride_b + ((long long)kvh * G + (valid ? n : 0)) * HD + q4 * 2;
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    qf[nt][kk][0] = valid ? *reinterpret_cast<const uint32_t*>(qp + kk * 16) : 0u;
-                    qf[nt][kk][1] = valid ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
-                }
-            }
-            float m[NT][2], l[NT][2];
-            float o[NT][HD / 16][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                m[nt][0] = m[nt][1] = -CUDART_INF_F;
-                l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-                for (int mt = 0; mt < HD / 16; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
-            }
-
+            group.load(p.q + b * p.q_stride_b + (long long)kvh * G * HD, G);
             for (int k0 = 0; k0 < seg; k0 += p.slices, ++it) {
                 const int st = it % p.stages;
-                if (!mbar_wait_warp(&full[st], (it / p.stages) & 1)) {
+                if (!mbar_wait_warp(&ring.full[st], (it / p.stages) & 1)) {
                     if (lane == 0) report_fault(p.fault, FAULT_WAIT_FULL, it);
                     ok = false;
                     break;
                 }
-                if (k0 + slice < seg) {
-                    const uint32_t vis = seen.keys_of(seen.slice(first + k0 + slice));
-                    // Swizzled addressing: 16-byte unit u of row r sits at unit u ^ (r & 7).
-                    const uint32_t sK = smem_u32(smem + (size_t)2 * st * tile_bytes) + slice * slice_bytes + hl * HEAD;
-                    const uint32_t sV = sK + tile_bytes;
-                    const int key_k = lane & 15, key_v = (lane & 7) + (lane >> 4) * 8;
-                    const uint32_t a_k = sK + key_k * 128, a_v = sV + key_v * 128;
-                    const int xk = key_k & 7, hk = lane >> 4;
-                    const int xv = key_v & 7, hv = (lane >> 3) & 1;
-                    if (vis != 0xffffu) {
-                        // Rows nobody sees may hold anything (never-written cache, another user's NaN): their V becomes zero, so
-                        // that 0 * x stays 0; their scores are replaced below.
-                        for (int u = lane; u < 16 * (HD / 8); u += 32) {
-                            const int key = u / (HD / 8), c = u % (HD / 8);
-                            if ((vis >> key) & 1u) continue;
-                            const uint32_t a = sV + (c >> 3) * CHUNK + key * 128 + (c & 7) * 16;  // (whole rows: their units' order does not matter)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0u) : "memory");
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    // Fragments are fetched AHEAD at a time and a batch before their MMAs (decode_sm100.cuh).
-                    constexpr int AHEAD = HD * NT > 256 ? 2 : 4, BATCHES = HD / 16 / AHEAD;
-                    constexpr int CHAINS = NT == 1 ? 4 : 2;  // independent sums of S
-                    uint32_t fr[2][AHEAD][4];
-                    auto fetch_k = [&](int bt) {
-#pragma unroll
-                        for (int e = 0; e < AHEAD; ++e) {
-                            const int kk = bt * AHEAD + e;
-                            ldmatrix_x4(fr[bt & 1][e], a_k + (kk >> 2) * CHUNK + ((((kk & 3) * 2 + hk) ^ xk) << 4));
-                        }
-                    };
-                    auto fetch_v = [&](int bt) {
-#pragma unroll
-                        for (int e = 0; e < AHEAD; ++e) {
-                            const int mt = bt * AHEAD + e;
-                            ldmatrix_x4_trans(fr[bt & 1][e], a_v + (mt >> 2) * CHUNK + ((((mt & 3) * 2 + hv) ^ xv) << 4));
-                        }
-                    };
-                    float acc[NT][CHAINS][4];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int hh = 0; hh < CHAINS; ++hh) acc[nt][hh][0] = acc[nt][hh][1] = acc[nt][hh][2] = acc[nt][hh][3] = 0.f;
-                    fetch_k(0);
-#pragma unroll
-                    for (int bt = 0; bt < BATCHES; ++bt) {
-                        if (bt + 1 < BATCHES) fetch_k(bt + 1);
-                        else if (NT == 1) fetch_v(0);  // (an even number of batches: into the other half)
-#pragma unroll
-                        for (int e = 0; e < AHEAD; ++e) {
-                            const int kk = bt * AHEAD + e;
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(acc[nt][kk % CHAINS], fr[bt & 1][e], qf[nt][kk][0], qf[nt][kk][1]);
-                        }
-                    }
-                    static_assert(BATCHES % 2 == 0, "the first batch of V goes where the last one of K is not");
-                    const bool v_lo = (vis >> g4) & 1u, v_hi = (vis >> (g4 + 8)) & 1u;
-                    uint32_t pb[NT][2];
-                    bool any_rescale = false;
-                    float alpha[NT][2];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float s = acc[nt][0][e] + acc[nt][1][e];
-                            if constexpr (CHAINS == 4) s += acc[nt][2][e] + acc[nt][3][e];
-                            s *= sl;
-                            x[e] = ((e < 2) ? v_lo : v_hi) ? s : -CUDART_INF_F;
-                        }
-                        float pr[4];
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            float mx = fmaxf(x[u], x[u + 2]);
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                            const float m_new = fmaxf(m[nt][u], mx);
-                            const float m_eff = (m_new == -CUDART_INF_F) ? 0.f : m_new;
-                            alpha[nt][u] = (m_new == -CUDART_INF_F) ? 1.f : fast_exp2(m[nt][u] - m_new);
-                            pr[u] = fast_exp2(x[u] - m_eff);
-                            pr[u + 2] = fast_exp2(x[u + 2] - m_eff);
-                            l[nt][u] = l[nt][u] * alpha[nt][u] + pr[u] + pr[u + 2];
-                            m[nt][u] = m_new;
-                            any_rescale |= alpha[nt][u] != 1.f;
-                        }
-                        pb[nt][0] = movmatrix_trans(pack_bf16x2(pr[0], pr[1]));
-                        pb[nt][1] = movmatrix_trans(pack_bf16x2(pr[2], pr[3]));
-                    }
-                    if (__any_sync(0xffffffffu, any_rescale)) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int mt = 0; mt < HD / 16; ++mt) {
-                                o[nt][mt][0] *= alpha[nt][0];
-                                o[nt][mt][1] *= alpha[nt][1];
-                                o[nt][mt][2] *= alpha[nt][0];
-                                o[nt][mt][3] *= alpha[nt][1];
-                            }
-                    }
-                    if (NT > 1) fetch_v(0);
-#pragma unroll
-                    for (int bt = 0; bt < BATCHES; ++bt) {
-                        if (bt + 1 < BATCHES) fetch_v(bt + 1);
-#pragma unroll
-                        for (int e = 0; e < AHEAD; ++e)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][bt * AHEAD + e], fr[bt & 1][e], pb[nt][0], pb[nt][1]);
-                    }
-                }
+                if (k0 + slice < seg)
+                    attend_slice<HD, NT>(group, smem_u32(ring.slice(st, 0, slice)) + hl * HEAD, smem_u32(ring.slice(st, 1, slice)) + hl * HEAD,
+                                         seen.keys_of(seen.slice(first + k0 + slice)), p.scale_log2);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[st]);
+                if (lane == 0) mbar_arrive(&ring.empty[st]);
             }
 
-            // Partial record of this (CTA, sequence, slice): normalised out + natural-log lse.  Those of the share's last segment are
-            // folded here first, into the record of slice 0 (decode_sm100.cuh).
-            const bool fold_here = p.slices > 1 && seg_end == g1;  // CTA-uniform
-            float* rec = reinterpret_cast<float*>(smem);               // [warp][NT * 8 heads][RS]
-            float* rec_lse = rec + (size_t)ncw * NT * 8 * RS;          // [warp][NT * 8]
-            if (fold_here) {
-                consumer_sync(ncw);  // every warp is through with the stages; no copy is in flight any more
-                folded = true;
-            }
-            if (ok) {
-                const long long part = ((long long)blockIdx.x + b) * p.slices + slice;
+            // Partial records: normalised out + natural-log lse.  Of the share's last segment (for most CTAs the only one) one, in
+            // slice 0's place; of a sequence that ends inside the share one per slice.  (With one slice a step there is nothing to
+            // fold: through shared memory all the same, a call took 1.4 us more.)
+            const long long part = ((long long)blockIdx.x + b) * p.slices;
+            if (p.slices > 1 && seg_end == g1) {  // CTA-uniform
+                if (!ok) break;
+                const long long row0 = part * p.nq + (long long)kvh * G;
+                fold_warps<HD, NT>(group, smem, ncw, p.nkv_cta, p.slices, hl, slice, G,
+                    [&](int n, int s, float mx, float z, float wt) {
+                        if (n < G && s == 0) p.part_lse[row0 + n] = z == 0.f ? -CUDART_INF_F : (mx + fast_log2(z)) * 0.6931471805599453f;
+                        return z == 0.f ? 0.f : __fdividef(wt, z);
+                    },
+                    [&](int n, int d, float4 v) { *reinterpret_cast<float4*>(p.part_o + (row0 + n) * HD + d) = v; });
+            } else if (ok) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float inv[2];
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        float ls = l[nt][u];
-                        ls += __shfl_xor_sync(0xffffffffu, ls, 4);
-                        ls += __shfl_xor_sync(0xffffffffu, ls, 8);
-                        ls += __shfl_xor_sync(0xffffffffu, ls, 16);
-                        inv[u] = ls == 0.f ? 0.f : 1.f / ls;  // (what is no number goes on to the result)
-                        const int n = nt * 8 + q4 * 2 + u;
-                        const float lse = ls == 0.f ? -CUDART_INF_F : (m[nt][u] + fast_log2(ls)) * 0.6931471805599453f;
-                        if (g4 == 0) {
-                            if (fold_here) rec_lse[warp * NT * 8 + n] = lse;
-                            else if (n < G) p.part_lse[part * p.nq + (long long)kvh * G + n] = lse;
-                        }
-                    }
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
+                        const float ls = group.sum(nt, u);
+                        const float inv = ls == 0.f ? 0.f : 1.f / ls;  // (what is no number goes on to the result)
                         const int n = nt * 8 + q4 * 2 + u;
-                        if (fold_here || n < G) {
-                            float* dst = fold_here ? rec + ((size_t)warp * NT * 8 + n) * RS
-                                                   : p.part_o + (part * p.nq + (long long)kvh * G + n) * HD;
+                        if (n >= G) continue;
+                        const long long row = (part + slice) * p.nq + (long long)kvh * G + n;
+                        if (g4 == 0) p.part_lse[row] = ls == 0.f ? -CUDART_INF_F : (group.m[nt][u] + fast_log2(ls)) * 0.6931471805599453f;
+                        float* dst = p.part_o + row * HD + g4;
 #pragma unroll
-                            for (int mt = 0; mt < HD / 16; ++mt) {
-                                dst[mt * 16 + g4] = o[nt][mt][u] * inv[u];
-                                dst[mt * 16 + g4 + 8] = o[nt][mt][u + 2] * inv[u];
-                            }
+                        for (int mt = 0; mt < HD / 16; ++mt) {
+                            dst[mt * 16] = group.o[nt][mt][u] * inv;
+                            dst[mt * 16 + 8] = group.o[nt][mt][u + 2] * inv;
                         }
                     }
-                }
-            }
-            if (fold_here) {
-                consumer_sync(ncw);  // all records of the CTA are in shared memory
-                const long long row0 = ((long long)blockIdx.x + b) * p.slices * p.nq + (long long)kvh * G;
-                for (int n = slice; n < G; n += p.slices) {
-                    const float li = lane < p.slices ? rec_lse[(lane * p.nkv_cta + hl) * NT * 8 + n] : -CUDART_INF_F;
-                    float mx = li;
-#pragma unroll
-                    for (int e = 4; e > 0; e >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, e));
-                    mx = __shfl_sync(0xffffffffu, mx, 0);
-                    if (mx == -CUDART_INF_F) mx = 0.f;  // (all empty, or no numbers)
-                    float z = __expf(li - mx);
-                    const float e0 = z;
-#pragma unroll
-                    for (int e = 4; e > 0; e >>= 1) z += __shfl_xor_sync(0xffffffffu, z, e);
-                    z = __shfl_sync(0xffffffffu, z, 0);
-                    const float weight = z == 0.f ? 0.f : e0 / z;
-                    float4 acc[HD / 128];
-#pragma unroll
-                    for (int j = 0; j < HD / 128; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int s = 0; s < p.slices; ++s) {
-                        const float wt = __shfl_sync(0xffffffffu, weight, s);
-                        const float* src = rec + ((size_t)(s * p.nkv_cta + hl) * NT * 8 + n) * RS + lane * 4;
-#pragma unroll
-                        for (int j = 0; j < HD / 128; ++j) {  // (an empty slice's record holds zeros)
-                            const float4 ov = *reinterpret_cast<const float4*>(src + 128 * j);
-                            acc[j].x = fmaf(wt, ov.x, acc[j].x);
-                            acc[j].y = fmaf(wt, ov.y, acc[j].y);
-                            acc[j].z = fmaf(wt, ov.z, acc[j].z);
-                            acc[j].w = fmaf(wt, ov.w, acc[j].w);
-                        }
-                    }
-                    const float rec_l = z == 0.f ? -CUDART_INF_F : mx + __logf(z);
-#pragma unroll
-                    for (int j = 0; j < HD / 128; ++j) *reinterpret_cast<float4*>(p.part_o + (row0 + n) * HD + lane * 4 + 128 * j) = acc[j];
-                    if (lane == 0) p.part_lse[row0 + n] = rec_l;
-                }
             }
             g = seg_end;
         }
-        // A warp that gave up a wait never reached the fold: it still meets the others at both barriers.
-        if (!folded && p.slices > 1) {
-            consumer_sync(ncw);
-            consumer_sync(ncw);
+        // A warp that gave up a wait does not fold: it meets the others at the fold's three barriers.
+        if (!ok && p.slices > 1)
+            for (int i = 0; i < 3; ++i) consumer_sync(ncw);
+    }
+}
+
+// One launch: a cluster of p.ncta CTAs (at most eight) owns a sequence (grid.z) and a group of KV heads (grid.y), its CTAs equal parts of the slices.
+// Each folds its warps' records and sends them, as they are, to the CTAs that finish the columns (the largest power of two of
+// the cluster's), which weight, gate and store them: no records in global memory, no merge.  The sends are st.async, counted by
+// an mbarrier of the CTA they go to, as in decode_sm100.cuh, whose comments have what was measured against a barrier of the
+// cluster.  Length and first pages are two trips in front of the first copy.
+template <int HD, int NT>
+__global__ void __launch_bounds__(288, 1)
+    sdpa_decode_paged_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                                     const DecodePagedParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int HEAD = HD / 64 * SLICE_CHUNK;
+
+    const int ncw = p.nkv_cta * p.slices;  // consumer warps
+    PagedRing ring;
+    ring.slice_bytes = p.nkv_cta * HEAD;
+    ring.tile_bytes = p.slices * ring.slice_bytes;
+    ring.base = smem;
+    ring.stages = p.stages;
+    ring.full = reinterpret_cast<uint64_t*>(smem + (size_t)p.stages * 2 * ring.tile_bytes);
+    ring.empty = ring.full + p.stages;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.z, rank = blockIdx.x, head0 = blockIdx.y * p.nkv_cta;
+    const int G = p.nq / p.nkv, rows = p.nkv_cta * G, rows2 = (rows + 1) & ~1;
+    const bool alone = p.ncta == 1;  // (st.async is for clusters: plain stores then)
+    // The CTAs that finish `dc` columns of all rows each; per CTA of the cluster they get [row][column], in front of them [CTA][row]
+    // maximum (log2 domain) and sum, and whether all of its waits ended well.
+    const int dc_log2 = (HD == 256 ? 8 : 7) - (31 - __clz(p.ncta)), dc = 1 << dc_log2, finishers = HD >> dc_log2;
+    uint64_t* gathered = ring.empty + p.stages;
+    int* gave_up = reinterpret_cast<int*>(gathered + 1);
+    float* cflag = reinterpret_cast<float*>(gathered + 2);     // [8]
+    float2* cml = reinterpret_cast<float2*>(cflag + 8);         // [8][rows2]
+    float* crec = reinterpret_cast<float*>(cml + 8 * rows2);    // [CTA][rows][dc]
+    float* cweight = crec + (size_t)p.ncta * rows * dc;         // [rows][8]
+    if (threadIdx.x == 32) {
+        prefetch_tensormap(&tm_k);
+        prefetch_tensormap(&tm_v);
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&ring.full[s], 1);
+            mbar_init(&ring.empty[s], ncw);
         }
+        mbar_init(gathered, 1);
+        *gave_up = 0;
+        fence_mbar_init();
+        mbar_arrive_expect_tx(gathered, (uint32_t)(p.ncta * (4 + rows * (8 + dc * 4))));
+    }
+    cluster_sync_all();  // every CTA runs: its shared memory may be written
+    // Up to here nothing depends on the kernels in front; everything below may.
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const uint32_t fault = threadIdx.x == 0 ? *reinterpret_cast<volatile uint32_t*>(p.fault) : 0u;
+    const int len = p.kv_len ? p.kv_len[b] : p.kv_len_uniform;
+    if (len > p.max_len) {  // (the same in all of the cluster's CTAs)
+        if (threadIdx.x == 0) report_fault(p.fault, FAULT_BAD_KV_RANGE, (uint32_t)b);
+        return;
+    }
+    const SeenKeys seen = seen_of(len, p.window, p.sinks);
+    // This CTA's slices [first, first + mine): whole steps as long as there are any.
+    const int steps_all = (seen.n + p.slices - 1) / p.slices, step0 = (int)((long long)steps_all * rank / p.ncta), step1 = (int)((long long)steps_all * (rank + 1) / p.ncta);
+    const int first = step0 * p.slices, mine = min(seen.n, step1 * p.slices) - first;
+
+    if (warp == ncw) {
+        // ------------------------------------------------------------------ producer
+        const int i = lane;
+        int page = 0, row = 0;
+        auto look_up = [&](int k0) {  // of this lane's slice of the step at k0
+            if (k0 + i >= mine || i >= p.slices) return;
+            const int key = seen.slice(first + k0 + i) * 16, column = key / p.page;
+            row = key - column * p.page;
+            page = p.table[b * p.table_stride + column];
+        };
+        look_up(0);
+        int it = 0;
+        for (int k0 = 0; k0 < mine; k0 += p.slices, ++it) {
+            const int own_page = page, own_row = row;
+            look_up(k0 + p.slices);
+            const int st = it % p.stages;
+            if (it >= p.stages && !mbar_wait_warp(&ring.empty[st], ((it / p.stages) - 1) & 1)) {
+                if (lane == 0) report_fault(p.fault, FAULT_WAIT_EMPTY, it);
+                break;
+            }
+            ask_slices(ring, tm_k, tm_v, p, st, min(p.slices, mine - k0), own_page, own_row, head0, b);
+        }
+        drain(ring, it);
+    } else if (warp < ncw) {
+        // ------------------------------------------------------------------ consumers
+        const int hl = warp % p.nkv_cta, slice = warp / p.nkv_cta, kvh = head0 + hl;
+        GroupState<HD, NT> group;
+        group.load(p.q + b * p.q_stride_b + (long long)kvh * G * HD, G);
+        bool ok = true;
+        int it = 0;
+        for (int k0 = 0; k0 < mine; k0 += p.slices, ++it) {
+            const int st = it % p.stages;
+            if (!mbar_wait_warp(&ring.full[st], (it / p.stages) & 1)) {
+                if (lane == 0) report_fault(p.fault, FAULT_WAIT_FULL, it);
+                ok = false;
+                break;
+            }
+            if (k0 + slice < mine)
+                attend_slice<HD, NT>(group, smem_u32(ring.slice(st, 0, slice)) + hl * HEAD, smem_u32(ring.slice(st, 1, slice)) + hl * HEAD,
+                                     seen.keys_of(seen.slice(first + k0 + slice)), p.scale_log2);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ring.empty[st]);
+        }
+        if (lane == 0 && (!ok || fault != 0u)) *reinterpret_cast<volatile int*>(gave_up) = 1;  // (no result is written)
+        const uint32_t bar = smem_u32(gathered);
+        fold_warps<HD, NT>(group, smem, ncw, p.nkv_cta, p.slices, hl, slice, G,
+            [&](int n, int s, float mx, float z, float wt) {
+                if (n < G && s < finishers) {
+                    float2* to = cml + rank * rows2 + hl * G + n;
+                    if (alone) *to = make_float2(mx, z);
+                    else st_async_f32x2(map_to_cta(smem_u32(to), s), make_float2(mx, z), map_to_cta(bar, s));
+                }
+                // (2^-6, taken back with the CTAs' weights: up to 64 records are added up before their sum of weights is divided by, and
+                // values that a record of its own can hold must not run over in between.)
+                return wt * 0.015625f;
+            },
+            [&](int n, int d, float4 v) {
+                float* at = crec + (size_t)(rank * rows + hl * G + n) * dc + (d & (dc - 1));
+                const int to = d >> dc_log2;
+                if (alone) *reinterpret_cast<float4*>(at) = v;
+                else st_async_f32x4(map_to_cta(smem_u32(at), to), v, map_to_cta(bar, to));
+            });
+        if (warp == 0 && lane < finishers) {  // (behind the fold's barriers: every warp has said whether it gave up)
+            const float good = *reinterpret_cast<volatile int*>(gave_up) ? 0.f : 1.f;
+            if (alone) cflag[0] = good;
+            else st_async_f32(map_to_cta(smem_u32(cflag + rank), lane), good, map_to_cta(bar, lane));
+        }
+    }
+    // This CTA's columns, two a thread, once every record is in its own shared memory.  (Nothing is sent to a CTA that finishes none, and
+    // what this one has sent is waited for by those it went to: no barrier of the cluster here.)
+    if (!alone && (rank << dc_log2) >= HD) return;
+    const int items = rows * (dc / 2);
+    auto offset_of = [&](int item) {
+        return (long long)b * p.o_stride_b + (long long)(head0 * G + (item >> (dc_log2 - 1))) * HD + rank * dc + (item & (dc / 2 - 1)) * 2;
+    };
+    uint32_t gw = p.gate && (int)threadIdx.x < items ? *reinterpret_cast<const uint32_t*>(p.gate + offset_of(threadIdx.x)) : 0u;
+    __syncwarp();
+    // Whether the records came is settled for the whole CTA before any warp goes on: each warp waits by its own clock.
+    const bool came = alone || mbar_wait_cluster(gathered, 0);
+    if (!__syncthreads_and(came)) {
+        if (!came && lane == 0) report_fault(p.fault, FAULT_WAIT_FULL, 0x10000u);
+        cluster_sync_all();  // (what is still under way here arrives before the other CTAs have gone)
+        return;
+    }
+    const bool fine = __all_sync(0xffffffffu, (lane & 7) >= p.ncta || cflag[lane & 7] != 0.f);  // (the same in every warp)
+    // The CTAs' weights of a row: eight lanes.
+#pragma unroll 1
+    for (int n0 = warp * 4; n0 < rows; n0 += (ncw + 1) * 4) {
+        const int n = n0 + (lane >> 3), c = lane & 7;
+        const float2 ml = n < rows && c < p.ncta ? cml[c * rows2 + n] : make_float2(-CUDART_INF_F, 0.f);
+        float mx = ml.y == 0.f ? -CUDART_INF_F : ml.x;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float wt = ml.y == 0.f ? 0.f : fast_exp2(ml.x - mx);
+        float z = wt * ml.y;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        if (n < rows) {
+            cweight[n * 8 + c] = z == 0.f ? 0.f : __fdividef(wt * 64.f, z);
+            if (p.out_lse && fine && rank == 0 && c == 0)
+                p.out_lse[(long long)b * p.nq + head0 * G + n] = z == 0.f ? -CUDART_INF_F : fmaf(mx, 0.6931471805599453f, logf(z));
+        }
+    }
+    __syncthreads();
+    if (!fine) return;
+#pragma unroll 1
+    for (int item = threadIdx.x; item < items; item += blockDim.x) {
+        const int n = item >> (dc_log2 - 1), d = (item & (dc / 2 - 1)) * 2;
+        const long long eoff = offset_of(item);
+        if (p.gate && item != (int)threadIdx.x) gw = *reinterpret_cast<const uint32_t*>(p.gate + eoff);
+        float a0 = 0.f, a1 = 0.f;
+#pragma unroll 2
+        for (int c = 0; c < p.ncta; ++c) {
+            const float wt = cweight[n * 8 + c];
+            const float2 v = *reinterpret_cast<const float2*>(crec + (size_t)(c * rows + n) * dc + d);
+            a0 = fmaf(wt, v.x, a0);
+            a1 = fmaf(wt, v.y, a1);
+        }
+        const long long row = (long long)b * p.nq + head0 * G + n;
+        if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * HD + rank * dc + d) = make_float2(a0, a1);
+        if (p.out) {
+            if (p.gate) a0 = gated<true>(a0, (uint16_t)(gw & 0xffffu)), a1 = gated<true>(a1, (uint16_t)(gw >> 16));
+            *reinterpret_cast<uint32_t*>(p.out + eoff) = pack_bf16x2(a0, a1);
+        }
+    }
+}
+
+// Merge of the records: a block takes ROWS query heads of a sequence, 8 / ROWS warps each.  What it costs is a chain of trips (the wait, the
+// log-sum-exps and values) and the blocks that stand in line for it, so where there are rows enough a warp takes one on its
+// own, and 64 registers let a block wait beside each decode CTA.  (48 sequences of 28 heads: 11.5 us as a block per row, which
+// is 4.5 waves of them.)  Rows of few sequences go by sdpa_decode_merge_kernel, whose blocks divide the columns, too.
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(256, ROWS == 1 ? 2 : 4) sdpa_decode_paged_merge_kernel(const DecodeMergeParams p) {
+    constexpr int TEAM = 8 / ROWS, VPL = HD / 32, U = HD == 256 ? 2 : 4;  // warps of a row; values of a lane; records a warp has in flight
+    __shared__ float s_acc[TEAM > 1 ? 8 * HD : 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x * ROWS + warp / TEAM, b = blockIdx.y, member = warp % TEAM;
+    // (The decode kernel released this one behind its own wait for the kernels in front: the lengths are final.)
+    long long k_begin = 0, total = 0, k_len = 0;
+    for (int i = lane; i < p.batch; i += 32) {
+        const int n = seen_of(p.kv_len ? p.kv_len[i] : p.kv_len_uniform, p.window, p.sinks).n;
+        total += n;
+        if (i < b) k_begin += n;
+        if (i == b) k_len = n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        k_begin += __shfl_xor_sync(0xffffffffu, k_begin, o);
+        k_len += __shfl_xor_sync(0xffffffffu, k_len, o);
+    }
+    const bool live = h < p.nq;
+    const long long eoff = (long long)b * p.o_stride_b + (long long)h * HD + lane * VPL;
+    if (p.gate && live) prefetch_l2(p.gate + eoff);
+    const long long per = share_size(total, p.ncta, p.slices), k_end = k_begin + k_len;
+    const bool small = total < (1ll << 30);
+    const int c_first = small ? (int)((uint32_t)k_begin / (uint32_t)per) : (int)(k_begin / per);
+    const int c_last = k_len == 0 ? c_first : small ? (int)((uint32_t)(k_end - 1) / (uint32_t)per) : (int)((k_end - 1) / per);
+    // The shares in front of the last one end with this sequence and have one record of it; the last one has one for each slice if
+    // it goes on behind it.
+    const int n_full = c_last - c_first;
+    const int n_rec = k_len == 0 || !live ? 0 : n_full + (k_end == min(total, (c_last + 1) * per) ? 1 : p.slices);
+    const long long part0 = ((long long)c_first + b) * p.slices;
+    auto rec_of = [&](int j) { return part0 + (j < n_full ? (long long)j * p.slices : (long long)n_full * p.slices + (j - n_full)); };
+    grid_dependency_wait();  // from here on the records are read
+    grid_launch_dependents();
+    const bool fault = *reinterpret_cast<volatile uint32_t*>(p.fault) != 0u;
+    const float* lses = p.part_lse + h;
+    float wu[U], acc[VPL];
+    float4 ov[U][VPL / 4];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * TEAM;
+            wu[u] = -CUDART_INF_F;
+            if (j < n_rec) {
+                const long long rec = rec_of(j);
+                wu[u] = lses[rec * p.nq];
+                const float* src = p.part_o + (rec * p.nq + h) * HD + lane * VPL;
+#pragma unroll
+                for (int i = 0; i < VPL / 4; ++i) ov[u][i] = *reinterpret_cast<const float4*>(src + 4 * i);
+            }
+        }
+    };
+    load(member);
+    float mx = -CUDART_INF_F, z = 0.f;
+    for (int j = lane; j < n_rec; j += 32) mx = fmaxf(mx, lses[rec_of(j) * p.nq]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (mx == -CUDART_INF_F) mx = 0.f;  // (no records, or none that are numbers)
+    for (int j = lane; j < n_rec; j += 32) z += __expf(lses[rec_of(j) * p.nq] - mx);  // (L1 has them)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
+    for (int j0 = member; j0 < n_rec; j0 += TEAM * U) {
+        if (j0 != member) load(j0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (wu[u] == -CUDART_INF_F) continue;  // an empty slice's record may hold anything
+            const float w = __expf(wu[u] - mx);
+#pragma unroll
+            for (int i = 0; i < VPL / 4; ++i) {
+                acc[4 * i] = fmaf(w, ov[u][i].x, acc[4 * i]), acc[4 * i + 1] = fmaf(w, ov[u][i].y, acc[4 * i + 1]);
+                acc[4 * i + 2] = fmaf(w, ov[u][i].z, acc[4 * i + 2]), acc[4 * i + 3] = fmaf(w, ov[u][i].w, acc[4 * i + 3]);
+            }
+        }
+    }
+    if constexpr (TEAM > 1) {
+#pragma unroll
+        for (int i = 0; i < VPL / 4; ++i)
+            *reinterpret_cast<float4*>(s_acc + warp * HD + lane * VPL + 4 * i) = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+        __syncthreads();
+        if (member != 0) return;
+#pragma unroll
+        for (int t = 1; t < TEAM; ++t)
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) acc[i] += s_acc[(warp + t) * HD + lane * VPL + i];
+    }
+    if (fault || !live) return;  // a status is set: no result
+    const float inv = z == 0.f ? 0.f : 1.f / z;
+    const long long row = (long long)b * p.nq + h;
+    if (p.out_lse && lane == 0) p.out_lse[row] = z == 0.f ? -CUDART_INF_F : mx + __logf(z);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) acc[i] *= inv;
+    if (p.out_f32) {
+#pragma unroll
+        for (int i = 0; i < VPL / 4; ++i)
+            *reinterpret_cast<float4*>(p.out_f32 + row * HD + lane * VPL + 4 * i) = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+    }
+    if (p.out) {
+        uint32_t o[VPL / 2];
+#pragma unroll
+        for (int i = 0; i < VPL / 2; ++i) {
+            if (p.gate) {
+                const uint32_t gw = *reinterpret_cast<const uint32_t*>(p.gate + eoff + 2 * i);
+                acc[2 * i] = gated<true>(acc[2 * i], (uint16_t)(gw & 0xffffu)), acc[2 * i + 1] = gated<true>(acc[2 * i + 1], (uint16_t)(gw >> 16));
+            }
+            o[i] = pack_bf16x2(acc[2 * i], acc[2 * i + 1]);
+        }
+        if constexpr (VPL == 8) *reinterpret_cast<uint4*>(p.out + eoff) = make_uint4(o[0], o[1], o[2], o[3]);
+        else *reinterpret_cast<uint2*>(p.out + eoff) = make_uint2(o[0], o[1]);
     }
 }
 

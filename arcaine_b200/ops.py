@@ -426,7 +426,8 @@ def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     without such a key are not looked at (their entries may be anything).  A sequence without keys gives zeros, lse -inf.
     Returns ``out`` (B, nq, hd) bf16, rounded once, after the gate; with ``return_partial`` also (out_f32, lse), ungated.
     A length beyond its table row, or an entry outside the pool, shows in ``device_status()`` (``FAULT_BAD_KV_RANGE``; detail:
-    the sequence), and the outputs are left unwritten.
+    the sequence), and the call's outputs are undefined.  The kernel is chosen by the table's width, which bounds the
+    lengths: pass no more columns (``block_table[:, :n]``) than the longest sequence may need.
     """
     return _native().sdpa_decode_paged(q, k_pages, v_pages, block_table, kv_len, scale, window, sinks, gate, out, return_partial,
                                        want_out, num_ctas, partial_out, partial_lse, workspace)

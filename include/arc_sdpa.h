@@ -388,7 +388,9 @@ int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void* stream);
  * token itself included) and the first `sinks`; pages that hold no such key are neither read nor looked up.  A sequence
  * without keys gives zeros and a log-sum-exp of -inf.  A kv_len beyond table_width * page_size, or an entry outside
  * [0, num_pages) for a page that is read, shows as ARC_ERR_DEVICE_BAD_RANGE in arc_sdpa_device_status() (detail: the
- * sequence) and leaves the outputs unwritten.  nq / nkv <= 16, batch <= 2048, hd 128 or 256. */
+ * sequence), and the call's outputs are undefined.  The table's width bounds the lengths, and by it the kernel is chosen (one
+ * launch or two): a table that is as wide as the longest sequence needs is the faster one.  nq / nkv <= 16, batch <= 2048,
+ * hd 128 or 256.  workspace: none where arc_sdpa_decode_paged_workspace_bytes() says 0. */
 typedef struct arc_sdpa_decode_paged_params {
     const void* q;       /* (batch, nq, hd) bf16, batch stride q_stride_b */
     const void* k_pages; /* (num_pages, page_size, nkv, hd) bf16 */

@@ -338,22 +338,24 @@ EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 100, 127, 128,
 
 
 @pytest.mark.parametrize("nq,nkv,hd", [(8, 4, 128), (24, 4, 256), (7, 7, 128), (16, 1, 128), (16, 2, 256), (28, 4, 128), (32, 16, 128), (4, 4, 256), (9, 3, 256)])
+@pytest.mark.parametrize("ctas", [0, 148])  # (0: the library's choice, here nearly always one launch; else two)
 @pytest.mark.parametrize("page,window,sinks", [(16, None, 0), (48, None, 3), (32, 20, 0), (64, 17, 4), (16, 1, 1), (256, 100, 40), (16, 33, 17), (128, 64, 1000)])
-def test_decode_edges(nq, nkv, hd, page, window, sinks):
+def test_decode_edges(nq, nkv, hd, page, window, sinks, ctas):
     """Lengths about the ends of slices and pages, behind windows and sinks of all sizes; what nobody sees is NaN and infinite."""
     from arcaine_b200 import ops
     scale = hd ** -0.5
+    launches = ops.launch_count()
     q, kp, vp, table, gate = paged_case(EDGES, page, nq, nkv, hd, window, sinks, seed=nq + page, interleave=page == 32)
     w = ops.NO_WINDOW if window is None else window
     want, want_lse, size = plain_decode(q, kp, vp, table, EDGES, window, sinks, scale)
-    out, o32, lse = ops.sdpa_decode_paged(q, kp, vp, table, ints(EDGES), scale=scale, window=w, sinks=sinks, return_partial=True)
-    assert ops.device_status() == (0, 0)
+    out, o32, lse = ops.sdpa_decode_paged(q, kp, vp, table, ints(EDGES), scale=scale, window=w, sinks=sinks, return_partial=True, num_ctas=ctas)
+    assert ops.device_status() == (0, 0) and ops.launch_count() - launches == (2 if ctas or (nkv == 16 and window is None) else 1)
     assert_attention(out, lse, want, want_lse, size)
     assert_attention(o32, None, want, want_lse, size, rounded=False)
     want, _, size = plain_decode(q, kp, vp, table, EDGES, window, sinks, scale, gate)
-    got = ops.sdpa_decode_paged(q, kp, vp, table, ints(EDGES), scale=scale, window=w, sinks=sinks, gate=gate)
+    got = ops.sdpa_decode_paged(q, kp, vp, table, ints(EDGES), scale=scale, window=w, sinks=sinks, gate=gate, num_ctas=ctas)
     assert_attention(got, None, want, want_lse, size)
-    again = ops.sdpa_decode_paged(q, kp, vp, table, ints(EDGES), scale=scale, window=w, sinks=sinks, gate=gate)
+    again = ops.sdpa_decode_paged(q, kp, vp, table, ints(EDGES), scale=scale, window=w, sinks=sinks, gate=gate, num_ctas=ctas)
     assert torch.equal(got, again)
 
 
@@ -393,13 +395,16 @@ def test_decode_infinite_and_missing_numbers_stay_in_their_row():
     lens = [700, 700, 700]
     q, kp, vp, table, _ = paged_case(lens, 16, 4, 2, 128, None, 0, seed=5)
     want = ops.sdpa_decode_paged(q, kp, vp, table, 700, scale=0.09)
-    bad = q.clone()
-    bad[1, 0, 5] = math.nan
-    out, _, lse = ops.sdpa_decode_paged(bad, kp, vp, table, 700, scale=0.09, return_partial=True)
-    assert bool(torch.isnan(out[1, 0]).all()) and bool(torch.isnan(lse[1, 0]))
-    keep = torch.ones(3, 4, dtype=torch.bool, device=DEV)
-    keep[1, 0] = False
-    assert torch.equal(out[keep], want[keep]) and bool(torch.isfinite(lse[keep]).all())
+    want2 = ops.sdpa_decode_paged(q, kp, vp, table, 700, scale=0.09, num_ctas=148)
+    for value in (math.nan, math.inf):
+        bad = q.clone()
+        bad[1, 0, 5] = value
+        for ctas, w in ((0, want), (148, want2)):
+            out, _, lse = ops.sdpa_decode_paged(bad, kp, vp, table, 700, scale=0.09, return_partial=True, num_ctas=ctas)
+            assert bool(torch.isnan(out[1, 0]).all()) and bool(torch.isnan(lse[1, 0]))
+            keep = torch.ones(3, 4, dtype=torch.bool, device=DEV)
+            keep[1, 0] = False
+            assert torch.equal(out[keep], w[keep]) and bool(torch.isfinite(lse[keep]).all())
 
 
 def test_decode_large_scores():
@@ -409,7 +414,12 @@ def test_decode_large_scores():
     q, kp, vp, table, _ = paged_case(lens, 16, 4, 1, 128, None, 0, seed=6, poison=False)
     q = (q.float() * 60).bfloat16()
     want, want_lse, size = plain_decode(q, kp, vp, table, lens, None, 0, 1.0)
-    out, _, lse = ops.sdpa_decode_paged(q, kp, vp, table, ints(lens), scale=1.0, return_partial=True)
+    for ctas in (0, 148):
+        out, _, lse = ops.sdpa_decode_paged(q, kp, vp, table, ints(lens), scale=1.0, return_partial=True, num_ctas=ctas)
+        large_scores_hold(out, lse, want, want_lse, size)
+
+
+def large_scores_hold(out, lse, want, want_lse, size):
     # a score is off by up to 128 products in fp32, of values up to 800: 2^-24 * 128 * 800 * 4 = 0.025, and so is the exponent
     assert bool(((lse.double() - want_lse).abs() <= 0.03).all())
     assert bool(((out.double() - want).abs() <= size * (2 * 0.026 + 2.0 ** -8) + want.abs() * 2.0 ** -8).all())
@@ -451,9 +461,10 @@ def test_decode_bad_pages_and_lengths(what):
     out = torch.full_like(q, 5.0)
     ops.sdpa_decode_paged(q, kp, vp, table, ints(lens), scale=1.0, out=out)
     assert ops.device_status() == (10, 1)
-    assert bool((out == 5.0).all())
-    ops.sdpa_decode_paged(q, kp, vp, table, ints([1, 1, 1]), scale=1.0, out=out)  # (nothing while the status is set)
-    assert bool((out == 5.0).all())
+    for sequences in (1, 3):  # (nothing while the status is set, in either form)
+        out.fill_(5.0)
+        ops.sdpa_decode_paged(q[:sequences], kp, vp, table[:sequences], ints([1] * sequences), scale=1.0, out=out[:sequences], num_ctas=3 - sequences)
+        assert bool((out == 5.0).all())
     ops.clear_device_status()
 
 
