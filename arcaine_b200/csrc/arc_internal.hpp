@@ -13,8 +13,10 @@ constexpr int kDecodeStaticSmem = 1024;
 struct HostState {
     uint32_t* fault;  // the status word kernels report to
     int sm_count, smem_optin;
+    int device;
     int decode_clusters[9];  // [size]: clusters of decode CTAs the device holds at once
 };
+constexpr int kMaxDevices = 64;
 int host_state(HostState* out);
 
 // Keeps the text of a failing CUDA call for arc_sdpa_last_error(); returns ARC_ERR_CUDA.

@@ -2,6 +2,7 @@
 #include "../../include/arc_sdpa.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -101,25 +102,29 @@ extern "C" int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void
     if ((rc = host_state(&hs)) != ARC_OK) return rc;
 
     QkvPagedParams kp{};
-    const void* src[3] = {p->q, p->k, p->v};
-    void* out[3] = {p->q_out, p->k_out, p->v_out};
-    void* pool[3] = {nullptr, p->k_pages, p->v_pages};
-    const int64_t src_stride[3] = {p->q_stride, p->k_stride, p->v_stride}, out_stride[3] = {p->q_out_stride, p->k_out_stride, p->v_out_stride};
-    const int64_t page_stride[3] = {0, p->k_stride_page, p->v_stride_page}, row_stride[3] = {0, p->k_stride_t, p->v_stride_t};
-    int rows = 0;
-    for (int i = 0; i < 3; ++i) {
-        if (src[i]) {
-            kp.src[i] = static_cast<const uint16_t*>(src[i]);
-            kp.out[i] = static_cast<uint16_t*>(out[i]);
-            kp.pages[i] = static_cast<uint16_t*>(pool[i]);
-            kp.src_stride[i] = src_stride[i];
-            kp.out_stride[i] = out_stride[i];
-            kp.page_stride[i] = page_stride[i];
-            kp.row_stride[i] = row_stride[i];
-            rows += i == 0 ? p->nq : p->nkv;
-        }
-        kp.end[i] = rows;
+    const auto u16 = [](const void* x) { return static_cast<uint16_t*>(const_cast<void*>(x)); };
+    kp.k0 = p->q ? p->nq : 0;
+    kp.v0 = kp.k0 + (p->k ? p->nkv : 0);
+    kp.rows = kp.v0 + (p->v ? p->nkv : 0);
+    if (p->q) {
+        kp.q = u16(p->q), kp.q_stride = p->q_stride;
+        kp.q_dst = u16(p->q_out), kp.q_dst_stride = p->q_out_stride;
     }
+    if (p->k) {
+        kp.k = u16(p->k), kp.k_stride = p->k_stride;
+        kp.pool_k = p->k_pages != nullptr;
+        kp.k_dst = u16(kp.pool_k ? p->k_pages : p->k_out);
+        kp.k_page_stride = p->k_stride_page, kp.k_row_stride = kp.pool_k ? p->k_stride_t : p->k_out_stride;
+        if (kp.pool_k) kp.k_also = u16(p->k_out), kp.k_also_stride = p->k_out_stride;
+    }
+    if (p->v) {
+        kp.v = u16(p->v), kp.v_stride = p->v_stride;
+        kp.pool_v = p->v_pages != nullptr;
+        kp.v_dst = u16(kp.pool_v ? p->v_pages : p->v_out);
+        kp.v_page_stride = p->v_stride_page, kp.v_row_stride = kp.pool_v ? p->v_stride_t : p->v_out_stride;
+        if (kp.pool_v) kp.v_also = u16(p->v_out), kp.v_also_stride = p->v_out_stride;
+    }
+    const int rows = kp.rows;
     kp.slots = pages ? p->slots : nullptr;
     kp.positions = p->positions;
     kp.inv_freq = p->inv_freq;
@@ -134,25 +139,21 @@ extern "C" int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void
     kp.norm_v = p->norm_v != 0;
     kp.eps = p->eps;
     kp.mscale = p->mscale;
-    // A warp takes a token at a time, or a part of a token's passes: whatever gives the last warp the fewest passes, the start of
-    // a unit (the token's angles) counted as one; whole tokens where there are several for every warp.
+    // Equal shares of all passes: a pass a warp while one CTA per SM has them all, then three and more (each CTA has its start to pay
+    // for: 128 tokens of 64 rows of 128, 2048 passes, 4.4 us as one each, 3.9 as two), on at most three CTAs per SM.
     const int passes = (rows + 512 / p->hd - 1) / (512 / p->hd);
-    const long long warps = (long long)hs.sm_count * 2 * PREP_WARPS;
-    int chunk = passes, chunks = 1;
-    long long best = 0;
-    for (int c = passes; p->tokens < 4 * warps; c = (c + 1) / 2) {
-        const int n = (passes + c - 1) / c;
-        const long long cost = ((long long)p->tokens * n + warps - 1) / warps * (c + 1);
-        if (best == 0 || cost < best) best = cost, chunk = c, chunks = n;
-        if (c == 1) break;
-    }
-    if ((long long)p->tokens * chunks + warps > 0x7fffffffLL) return ARC_ERR_TOO_LARGE;
-    const long long units = (long long)p->tokens * chunks;
-    const unsigned ctas = (unsigned)((std::min(units, warps) + PREP_WARPS - 1) / PREP_WARPS);
+    const long long total = (long long)p->tokens * passes, one_each = (long long)hs.sm_count * PREP_WARPS;
+    if (total > 0x7fffffffLL) return ARC_ERR_TOO_LARGE;
+    const long long warps = total <= one_each ? total : std::min(3 * one_each, std::max(one_each, total / 3));
+    const unsigned ctas = (unsigned)((warps + PREP_WARPS - 1) / PREP_WARPS);
+    const int share = (int)(total / ((long long)ctas * PREP_WARPS)), longer = (int)(total % ((long long)ctas * PREP_WARPS));
+    const bool common = kp.norm_qk && !kp.norm_v && kp.pool_k && kp.pool_v && !kp.k_also && !kp.v_also;
     auto launch = [&](auto hd_tag) {
         constexpr int H = decltype(hd_tag)::value;
-        return launch_dependent(p->interleaved ? qkv_prepare_paged_kernel<H, true> : qkv_prepare_paged_kernel<H, false>, dim3(ctas), dim3(32 * PREP_WARPS), 0,
-                                static_cast<cudaStream_t>(stream), 1, kp, chunk, chunks);
+        const auto kernel = common ? (p->interleaved ? qkv_prepare_paged_kernel<H, true, true> : qkv_prepare_paged_kernel<H, false, true>)
+                                   : (p->interleaved ? qkv_prepare_paged_kernel<H, true, false> : qkv_prepare_paged_kernel<H, false, false>);
+        return launch_dependent(kernel, dim3(ctas), dim3(32 * PREP_WARPS), 0,
+                                static_cast<cudaStream_t>(stream), 1, kp, passes, share, longer);
     };
     ARC_CUDA(p->hd == 128 ? launch(std::integral_constant<int, 128>{}) : p->hd == 256 ? launch(std::integral_constant<int, 256>{}) : launch(std::integral_constant<int, 512>{}));
     count_launch();
@@ -264,10 +265,28 @@ static int make_pool_map(CUtensorMap* tm, const void* base, int hd, int nkv, int
     return encode_bf16_map(tm, base, 5, dims, strides, box, " (pages)");
 }
 
+// Dynamic shared memory beyond 48 KB, once per device: a call of its own for every launch took 0.6 us.
+static int allow_shared_memory(const HostState& hs) {
+    static std::atomic<bool> done[kMaxDevices];
+    if (done[hs.device].load(std::memory_order_acquire)) return ARC_OK;
+    const int most = hs.smem_optin - kDecodeStaticSmem;
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<128, 1>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<128, 2>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<256, 1>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<256, 2>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<128, 1>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<128, 2>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<256, 1>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<256, 2>, most));
+    done[hs.device].store(true, std::memory_order_release);
+    return ARC_OK;
+}
+
 template <int HD>
 static int launch_decode_paged(const arc_sdpa_decode_paged_params* p, const DecodePagedPlan& plan, const HostState& hs, cudaStream_t stream) {
     CUtensorMap tk, tv;
     int rc;
+    if ((rc = allow_shared_memory(hs)) != ARC_OK) return rc;
     if ((rc = make_pool_map(&tk, p->k_pages, HD, p->nkv, plan.nkv_cta, p->page_size, p->num_pages, p->k_stride_t, p->k_stride_page)) != ARC_OK) return rc;
     if ((rc = make_pool_map(&tv, p->v_pages, HD, p->nkv, plan.nkv_cta, p->page_size, p->num_pages, p->v_stride_t, p->v_stride_page)) != ARC_OK) return rc;
     DecodePagedParams kp{};
@@ -300,14 +319,12 @@ static int launch_decode_paged(const arc_sdpa_decode_paged_params* p, const Deco
         kp.out_lse = p->out_lse;
         kp.o_stride_b = p->o_stride_b;
         const auto kernel = plan.nt == 1 ? sdpa_decode_paged_cluster_kernel<HD, 1> : sdpa_decode_paged_cluster_kernel<HD, 2>;
-        ARC_CUDA(opt_in_smem(kernel, hs.smem_optin - kDecodeStaticSmem));
         ARC_CUDA(launch_dependent(kernel, dim3((unsigned)plan.ncta, (unsigned)plan.groups, (unsigned)p->batch), dim3(32u * (unsigned)(plan.nkv_cta * plan.slices + 1)),
                                   (size_t)plan.smem_bytes, stream, plan.ncta, tk, tv, kp));
         count_launch();
         return ARC_OK;
     }
     const auto kernel = plan.nt == 1 ? sdpa_decode_paged_kernel<HD, 1> : sdpa_decode_paged_kernel<HD, 2>;
-    ARC_CUDA(opt_in_smem(kernel, hs.smem_optin - kDecodeStaticSmem));
     ARC_CUDA(launch_dependent(kernel, dim3((unsigned)plan.ncta, (unsigned)plan.groups), dim3(32u * (unsigned)(plan.nkv_cta * plan.slices + 1)),
                               (size_t)plan.smem_bytes, stream, 1, tk, tv, kp));
     count_launch();
@@ -356,7 +373,7 @@ extern "C" int arc_sdpa_decode_paged(const arc_sdpa_decode_paged_params* p, void
     if (!p || !p->q || !p->k_pages || !p->v_pages || !p->block_table || (!p->out && !p->out_f32) || (p->gate && !p->out)) return ARC_ERR_NULL_POINTER;
     // What needs no device is refused without one.
     DecodePagedPlan plan;
-    int rc = plan_decode_paged(p, HostState{nullptr, 148, 232448, {}}, &plan);
+    int rc = plan_decode_paged(p, HostState{nullptr, 148, 232448, 0, {}}, &plan);
     if (rc != ARC_OK) return rc;
     if (!aligned16(p->q) || !aligned16(p->k_pages) || !aligned16(p->v_pages) || !aligned16(p->out) || !aligned16(p->gate) || !aligned16(p->out_f32) ||
         ((reinterpret_cast<uintptr_t>(p->block_table) | reinterpret_cast<uintptr_t>(p->kv_len) | reinterpret_cast<uintptr_t>(p->out_lse)) & 3u) ||

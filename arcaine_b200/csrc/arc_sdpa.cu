@@ -30,7 +30,6 @@ namespace arc {
 // Per-device status word written by kernels whose bounded waits give up.
 __device__ uint32_t g_fault_words[2];
 
-constexpr int kMaxDevices = 64;
 
 // What the device holds of the CTA pairs of prefill_wide_sm100.cuh at once (the defaults: a B200).
 struct WideRoom {
@@ -188,7 +187,7 @@ int host_state(HostState* out) {
     DeviceState* ds = nullptr;
     const int rc = device_state(&ds);
     if (rc != ARC_OK) return rc;
-    *out = HostState{ds->fault, ds->sm_count, ds->smem_optin, {}};
+    *out = HostState{ds->fault, ds->sm_count, ds->smem_optin, (int)(ds - g_dev), {}};
     std::copy(std::begin(ds->decode_clusters), std::end(ds->decode_clusters), out->decode_clusters);
     return ARC_OK;
 }

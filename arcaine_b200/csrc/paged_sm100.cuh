@@ -135,60 +135,96 @@ __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const Page
 }
 
 struct QkvPagedParams {
-    const uint16_t* src[3];  // projected rows of Q, K, V: (tokens, heads, hd)
-    uint16_t* out[3];        // rows for the caller, or nullptr
-    uint16_t* pages[3];      // the pools of K and V, or nullptr
+    const uint16_t *q, *k, *v;    // projected rows: (tokens, heads, hd); nullptr: none
+    uint16_t *q_dst, *k_dst, *v_dst;  // rows of Q; of K and V the pools where there are any (PAGES_K, PAGES_V), else rows
+    uint16_t *k_also, *v_also;    // rows of K and V besides the pools, or nullptr
     const int* slots;
     const int* positions;
     const double* inv_freq;
     const uint16_t* weight[2];
     uint32_t* fault;
     int tokens, page, num_rows;  // num_rows: of a pool
-    int end[3];                  // first row of a token behind its Q / K / V rows
+    int k0, v0, rows;            // a token's first K row, first V row, all its rows
     int half;                    // rotary_dim / 2
-    int norm_qk, norm_v;
-    long long src_stride[3], out_stride[3], page_stride[3], row_stride[3];
+    int norm_qk, norm_v, pool_k, pool_v;  // pool_*: k_dst / v_dst is a pool
+    long long q_stride, k_stride, v_stride, q_dst_stride, k_also_stride, v_also_stride;
+    long long k_page_stride, v_page_stride, k_row_stride, v_row_stride;  // row stride: between two rows of a page, or two tokens
     float eps, mscale;
 };
 
-// A warp takes a token, or a part of its rows where tokens are few, 512 / HD rows a pass: a lane holds two 16-byte pieces of a row
-// such that no rotation pair leaves it.  With r = rotary_dim / 16 lanes that rotate, those are pieces (l, l + r) for l < r and
-// (2 l, 2 l + 1) for the others in the half layout, (2 l, 2 l + 1) for all in the interleaved one; either way lane l < r has the
-// pairs 8 l to 8 l + 7.  Norm and rotation stay in fp32 and are rounded once.
+// A pass is 512 / HD rows of a token by a warp.  All tokens' passes are laid end to end and cut into equal parts, one per warp, which may
+// begin and end inside a token (whole tokens in turn left a tenth of the last round idle).  A lane holds two 16-byte pieces of a row
+// such that no rotation pair leaves it, and a load's pieces lie side by side.  Half layout, r = rotary_dim / 16: pieces l and l + r for
+// the lanes l < r, which have the pairs 8 l to 8 l + 7, and l + r and l + HD / 16 for the others.  Interleaved: pieces l and
+// l + HD / 16, each with its own four pairs.  Norm and rotation stay in fp32 and are rounded once.
 //
 // Angles: turns = position * inv_freq / 2 pi in 64 bits, less the nearest whole number; what is left, at most half a turn, is exact
 // in fp32 and goes to sincospif.  (In fp32 the angle of position 500000 would be off by 0.03 rad.)  Once a token and pair, not a head.
-template <int HD, bool INTERLEAVED>
-__global__ void __launch_bounds__(32 * PREP_WARPS, 2) qkv_prepare_paged_kernel(const QkvPagedParams p, const int chunk, const int chunks) {
+//
+// Bound by HBM, reads and writes mixed; a pass's rows are asked for one ahead, over the end of a token, too, and with them the
+// next token's position and slot.  (16384 tokens of 32/16 heads of 128, 537 MB: 149 us asked for when needed, two CTAs an SM.)
+// passes: of a token; share: passes of a warp, one more for the first `longer` of them.  COMMON: Q and K rows normed, V rows copied, K and V to pools only.
+template <int HD, bool INTERLEAVED, bool COMMON>
+__global__ void __launch_bounds__(32 * PREP_WARPS, 3) qkv_prepare_paged_kernel(const QkvPagedParams p, const int passes, const int share, const int longer) {
     constexpr int LPR = HD / 16;   // lanes per row
     constexpr int RPW = 512 / HD;  // rows per pass
     __shared__ __align__(16) float s_cos[PREP_WARPS][HD / 2], s_sin[PREP_WARPS][HD / 2];
     __shared__ __align__(16) float s_w[2][HD];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int sub = lane / LPR, li = lane % LPR;
-    const int turning = p.half >> 3;  // lanes of a row that rotate
-    const bool split = !INTERLEAVED && li < turning;
-    const int c0 = (split ? li : 2 * li) * 8, c1 = (split ? li + turning : 2 * li + 1) * 8;  // this lane's columns
+    const int turning = p.half >> 3;  // half layout: lanes of a row that rotate
+    const bool second = !INTERLEAVED && li >= turning;  // (that do not)
+    const int c0 = (second ? li + turning : li) * 8;    // this lane's columns: [c0, c0 + 8) and `apart` on
+    const int apart = INTERLEAVED ? HD / 2 : second ? HD / 2 - turning * 8 : turning * 8;
+    const int pair0 = INTERLEAVED ? li * 4 : li * 8, pair1 = INTERLEAVED ? pair0 + HD / 4 : pair0 + 4;  // four pairs each
+    const bool norm_qk = COMMON || p.norm_qk, norm_v = !COMMON && p.norm_v, pool_k = COMMON || p.pool_k, pool_v = COMMON || p.pool_v, slots = COMMON || p.slots;
     grid_dependency_wait();
     grid_launch_dependents();
     for (int i = threadIdx.x; i < 2 * HD; i += blockDim.x) {
         const uint16_t* w = p.weight[i / HD];
         s_w[i / HD][i % HD] = w ? bf16_bits_to_f32(w[i % HD]) : 1.0f;
     }
-    const bool aborted = __syncthreads_or(threadIdx.x == 0 && *reinterpret_cast<volatile uint32_t*>(p.fault) != 0u);
-    if (aborted) return;  // a status is set: no work
-    const int units = p.tokens * chunks;  // the host keeps this below 2^31
-    for (int u = blockIdx.x * PREP_WARPS + warp; u < units; u += gridDim.x * PREP_WARPS) {
-        const int t = u / chunks, r_begin = (u - t * chunks) * chunk * RPW, r_end = min(p.end[2], r_begin + chunk * RPW);
-        const int pos = p.positions[t];
-        if (pos < 0) continue;  // padding
-        int slot = p.slots ? p.slots[t] : -1;
-        if (slot >= p.num_rows || slot < -1) {
-            if (p.slots && lane == 0) report_fault(p.fault, FAULT_BAD_KV_RANGE, (uint32_t)t);
+    const int w = blockIdx.x * PREP_WARPS + warp;
+    int left = share + (w < longer ? 1 : 0);  // passes of this warp to be worked on
+    const int at = w * share + min(w, longer);
+
+    // The walk of the loads, a pass ahead of the work: token ft, rows from fr to f_end; f_left passes to be asked for.
+    int ft = at / passes, fr = (at - ft * passes) * RPW, f_left = left, f_pos = -1, f_slot = -1;
+    const uint16_t *fq = nullptr, *fk = nullptr, *fv = nullptr;
+    auto begin_loads = [&]() {
+        f_pos = p.positions[ft];
+        f_slot = slots ? p.slots[ft] : 0;
+        fq = p.q + ft * p.q_stride + c0;
+        fk = p.k + ft * p.k_stride + c0 - p.k0 * HD;
+        fv = p.v + ft * p.v_stride + c0 - p.v0 * HD;
+    };
+    uint4 na = make_uint4(0u, 0u, 0u, 0u), nb = na;
+    auto fetch = [&]() {
+        const int r = fr + sub;
+        if (r < p.rows) {
+            const uint16_t* src = (r < p.k0 ? fq : r < p.v0 ? fk : fv) + r * HD;
+            na = *reinterpret_cast<const uint4*>(src);
+            nb = *reinterpret_cast<const uint4*>(src + apart);
+        }
+        fr += RPW;
+        --f_left;
+    };
+    int t = ft, r0 = fr;
+    if (left > 0) {
+        begin_loads();
+        fetch();
+    }
+    if (__syncthreads_or(threadIdx.x == 0 && *reinterpret_cast<volatile uint32_t*>(p.fault) != 0u)) return;  // a status is set: no work
+
+    for (; left > 0; ++t, r0 = 0) {
+        const int pos = f_pos;
+        int slot = f_slot;
+        if (slots && (slot >= p.num_rows || slot < -1)) {
+            if (lane == 0 && pos >= 0) report_fault(p.fault, FAULT_BAD_KV_RANGE, (uint32_t)t);
             slot = -1;
         }
-        const int page = slot < 0 ? 0 : slot / p.page, row = slot - page * p.page;
-        if (r_begin < p.end[1] && p.half > 0) {
+        const bool live = pos >= 0, stored = live && slot >= 0;  // (padding; rows that are not appended)
+        if (live && r0 < p.v0 && p.half > 0) {
             __syncwarp();
             for (int f = lane; f < p.half; f += 32) {
                 const double turns = (double)pos * p.inv_freq[f] * 0.15915494309189533577;
@@ -199,63 +235,88 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 2) qkv_prepare_paged_kernel(c
             }
             __syncwarp();
         }
-        for (int r0 = r_begin; r0 < r_end; r0 += RPW) {
-            const int r = r0 + sub;
-            const bool there = r < r_end;
-            const int part = r < p.end[0] ? 0 : r < p.end[1] ? 1 : 2, head = r - (part ? p.end[part - 1] : 0);
-            uint4 ra = make_uint4(0u, 0u, 0u, 0u), rb = ra;
-            if (there) {
-                const uint16_t* src = p.src[part] + t * p.src_stride[part] + (long long)head * HD;
-                ra = *reinterpret_cast<const uint4*>(src + c0);
-                rb = *reinterpret_cast<const uint4*>(src + c1);
+        const int page = stored && slots ? slot / p.page : 0, row = slots ? slot - page * p.page : t;
+        uint16_t* dq = p.q_dst + t * p.q_dst_stride + c0;
+        uint16_t* dk = p.k_dst + (pool_k ? page * p.k_page_stride + row * p.k_row_stride : t * p.k_row_stride) + c0 - p.k0 * HD;
+        uint16_t* dv = p.v_dst + (pool_v ? page * p.v_page_stride + row * p.v_row_stride : t * p.v_row_stride) + c0 - p.v0 * HD;
+        for (; left > 0 && r0 < p.rows; r0 += RPW, --left) {
+            uint4 ra = na, rb = nb;
+            if (f_left > 0) {
+                if (fr >= p.rows) {  // the next token's first rows follow at once
+                    ++ft, fr = 0;
+                    begin_loads();
+                }
+                fetch();
             }
-            if (part == 2 ? p.norm_v : (p.norm_qk || p.half)) {
+            const int r = r0 + sub;
+            const bool is_v = r >= p.v0;
+            if (r0 >= p.v0 ? norm_v : (norm_qk || norm_v || p.half)) {  // (what only V rows share with the pass is copied below)
                 float a[8], b[8];
                 unpack8(ra, a);
                 unpack8(rb, b);
-                float ss = 0.f;
+                if (norm_qk || norm_v) {
+                    float ss = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
-                // (a row's lanes agree on its part)
-                const uint32_t row_lanes = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (sub * LPR);
+                    for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
 #pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(row_lanes, ss, o);
-                if (part == 2 || p.norm_qk) {
-                    const float inv = rsqrtf(ss / static_cast<float>(HD) + p.eps);
+                    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const float inv = (is_v ? norm_v : norm_qk) ? rsqrtf(ss / static_cast<float>(HD) + p.eps) : 1.0f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) a[e] *= inv, b[e] *= inv;
-                    if (part < 2) {
-                        const float *wa = s_w[part] + c0, *wb = s_w[part] + c1;
+                    if (r0 < p.v0 && norm_qk && !is_v) {
+                        const float* w = s_w[r < p.k0 ? 0 : 1] + c0;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) a[e] *= wa[e], b[e] *= wb[e];
+                        for (int e = 0; e < 8; e += 4) {
+                            const float4 x = *reinterpret_cast<const float4*>(w + e), y = *reinterpret_cast<const float4*>(w + apart + e);
+                            a[e] *= x.x, a[e + 1] *= x.y, a[e + 2] *= x.z, a[e + 3] *= x.w;
+                            b[e] *= y.x, b[e + 1] *= y.y, b[e + 2] *= y.z, b[e + 3] *= y.w;
+                        }
                     }
                 }
-                if (part < 2 && li < turning) {
-                    const float *cs = s_cos[warp] + li * 8, *sn = s_sin[warp] + li * 8;
+                if (pair0 < p.half && !is_v) {
+                    float c[8], s[8];  // (interleaved: of pair1 on whatever is there, where those do not rotate)
+                    auto angles = [&](const float* from, float* to, int pair) {
+                        const float4 x = *reinterpret_cast<const float4*>(from + pair);
+                        to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+                    };
+                    angles(s_cos[warp], c, pair0), angles(s_cos[warp], c + 4, pair1);
+                    angles(s_sin[warp], s, pair0), angles(s_sin[warp], s + 4, pair1);
                     auto turn = [&](float& x, float& y, int f) {
                         const float x0 = x, y0 = y;
-                        x = x0 * cs[f] - y0 * sn[f];
-                        y = x0 * sn[f] + y0 * cs[f];
+                        x = x0 * c[f] - y0 * s[f];
+                        y = x0 * s[f] + y0 * c[f];
                     };
+                    if constexpr (INTERLEAVED) {
 #pragma unroll
-                    for (int f = 0; f < 8; ++f) {
-                        if constexpr (INTERLEAVED) turn(f < 4 ? a[2 * f] : b[2 * f - 8], f < 4 ? a[2 * f + 1] : b[2 * f - 7], f);
-                        else turn(a[f], b[f], f);
+                        for (int f = 0; f < 4; ++f) turn(a[2 * f], a[2 * f + 1], f);
+                        if (pair1 < p.half) {
+#pragma unroll
+                            for (int f = 0; f < 4; ++f) turn(b[2 * f], b[2 * f + 1], f + 4);
+                        }
+                    } else {
+#pragma unroll
+                        for (int f = 0; f < 8; ++f) turn(a[f], b[f], f);
                     }
                 }
-                ra = pack8(a);
-                rb = pack8(b);
+                if (!is_v || norm_v) {
+                    ra = pack8(a);
+                    rb = pack8(b);
+                }
             }
-            if (!there) continue;
-            if (p.out[part]) {
-                uint16_t* dst = p.out[part] + t * p.out_stride[part] + (long long)head * HD;
-                *reinterpret_cast<uint4*>(dst + c0) = ra;
-                *reinterpret_cast<uint4*>(dst + c1) = rb;
+            if (r >= p.rows || !live) continue;
+            const bool is_q = r < p.k0;
+            if (is_q || stored || !(is_v ? pool_v : pool_k)) {
+                uint16_t* dst = (is_q ? dq : is_v ? dv : dk) + r * HD;
+                *reinterpret_cast<uint4*>(dst) = ra;
+                *reinterpret_cast<uint4*>(dst + apart) = rb;
             }
-            if (p.pages[part] && slot >= 0) {
-                uint16_t* dst = p.pages[part] + page * p.page_stride[part] + row * p.row_stride[part] + (long long)head * HD;
-                *reinterpret_cast<uint4*>(dst + c0) = ra;
-                *reinterpret_cast<uint4*>(dst + c1) = rb;
+            if (!COMMON && !is_q && (p.k_also || p.v_also)) {
+                uint16_t* also = is_v ? p.v_also : p.k_also;
+                if (also) {
+                    also += t * (is_v ? p.v_also_stride : p.k_also_stride) + (r - (is_v ? p.v0 : p.k0)) * HD + c0;
+                    *reinterpret_cast<uint4*>(also) = ra;
+                    *reinterpret_cast<uint4*>(also + apart) = rb;
+                }
             }
         }
     }
