@@ -485,6 +485,7 @@ static int launch_prefill(const arc_sdpa_prefill_params* p, const PrefillPlan& p
     kp.mask_type = p->mask_type;
     kp.window = p->window;
     kp.sinks = sinks_of(p);
+    kp.sink_blocks = (kp.sinks + 127) / 128;
     const bool sinks = p->sinks > 0;  // (also where they change nothing: how a gated result is rounded goes by the argument)
     kp.num_splits = plan.splits;
     kp.group = p->nq / p->nkv;

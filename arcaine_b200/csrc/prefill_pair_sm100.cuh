@@ -83,13 +83,18 @@ struct PairWork {
     int b, kvh;
     int lo[2], hi[2];
     int ulo, uhi;  // union of the two ranges (contiguous)
-    int gap;  // SINKS (key_block)
+    int gap;       // SINKS: the union's window begins there; blocks [ulo, gap) are those of the sinks, which both tiles see
     bool live[2];  // the tile has rows below seq
     // Selected without dynamic indexing, so the struct stays in registers.
     __device__ __forceinline__ int q0_of(int s) const { return s ? q0[1] : q0[0]; }
     __device__ __forceinline__ int h_of(int s) const { return s ? h[1] : h[0]; }
     __device__ __forceinline__ int lo_of(int s) const { return s ? lo[1] : lo[0]; }
     __device__ __forceinline__ int hi_of(int s) const { return s ? hi[1] : hi[0]; }
+    // A tile's first block, and whether it sees block j of the union.
+    template <bool SINKS>
+    __device__ __forceinline__ int first_of(int s) const { return SINKS && ulo < gap ? ulo : lo_of(s); }
+    template <bool SINKS>
+    __device__ __forceinline__ bool sees(int s, int j) const { return j < hi_of(s) && (j >= lo_of(s) || (SINKS && j < gap)); }
     __device__ __forceinline__ bool live_of(int s) const { return s ? live[1] : live[0]; }
 };
 
@@ -154,7 +159,7 @@ __device__ __forceinline__ void tile_blocks(const PrefillParams& p, int qs, int&
 // Keys that stay visible behind a window (sinks): their blocks go in front of the window's, which begin at block `lo`, and all roles
 // count them as blocks right ahead of it, from sinks_begin(lo) on.  So nothing but loads and masks knows that they are elsewhere.
 // (A tile that sees nothing has lo = 0.)
-__device__ __forceinline__ int sinks_begin(const PrefillParams& p, int lo) { return lo - min((p.sinks + 127) >> 7, lo); }
+__device__ __forceinline__ int sinks_begin(const PrefillParams& p, int lo) { return lo - min(p.sink_blocks, lo); }
 // The keys' block that is block j of a tile whose window begins at block `gap`.
 __device__ __forceinline__ int key_block(const PrefillParams& p, int j, int gap) { return j < gap ? j - sinks_begin(p, gap) : j; }
 
@@ -193,12 +198,9 @@ __device__ __forceinline__ PairWork decode_pair(const PrefillParams& p, const Ti
             }
     }
     if (t.uhi == 0) t.ulo = 0;
-    if constexpr (SINKS) {  // (the second tile's blocks, too, from the first one's window on: what it does not see is masked)
+    if constexpr (SINKS) {
         t.gap = t.ulo;
         t.ulo = sinks_begin(p, t.gap);
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-            if (t.hi[s] > t.lo[s]) t.lo[s] = t.ulo;
     }
     return t;
 }
@@ -213,9 +215,14 @@ __device__ __forceinline__ void mask_chunk(uint32_t (&v)[32], int key0, const Ro
 }
 
 // The same where keys [0, sinks) are visible, too.
+__device__ __forceinline__ uint32_t bits_from(int pos, int n) {  // n bits from bit pos on, cut off at bit 32
+    uint32_t m;
+    asm("bmsk.clamp.b32 %0, %1, %2;" : "=r"(m) : "r"(pos), "r"(n));
+    return m;
+}
 __device__ __forceinline__ void mask_chunk(uint32_t (&v)[32], int key0, const RowMask& rm, int sinks) {
-    const int lo = min(max(rm.lo - key0, 0), 32), hi = min(max(rm.hi - key0, 0), 32), first = min(max(sinks - key0, 0), 32);
-    const uint32_t vis = (uint32_t)(((1ull << hi) - (1ull << lo)) | ((1ull << first) - 1ull));
+    const int lo = max(rm.lo - key0, 0);
+    const uint32_t vis = bits_from(lo, max(rm.hi - key0 - lo, 0)) | bits_from(0, max(sinks - key0, 0));
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] = (vis >> e) & 1u ? v[e] : 0xff800000u;
 }
@@ -462,7 +469,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
             auto load = [&](uint8_t* dst, const void* tm, uint64_t* bar, const PairWork& pw, int j) {
 #pragma unroll
                 for (int c = 0; c < C::CH; ++c)
-                    tma_load_4d_warp(dst + c * C::CHUNK_BYTES, tm, bar, c * 64, pw.kvh, (SINKS ? key_block(p, j, pw.gap) : j) * C::BN, pw.b);
+                    tma_load_4d_warp(dst + c * C::CHUNK_BYTES, tm, bar, c * 64, pw.kvh, (SINKS && j < pw.gap ? j - pw.ulo : j) * C::BN, pw.b);
             };
             TileCursor cur = *cursor;
             PairWork last{};  // unit and index of the block requested last
@@ -576,8 +583,8 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                     }
 #pragma unroll 1
                     for (int s = 0; s < 2; ++s) {
-                        if (j < pw.lo_of(s) || j >= pw.hi_of(s)) continue;
-                        if (j == pw.lo_of(s)) {
+                        if (!pw.sees<SINKS>(s, j)) continue;
+                        if (j == pw.first_of<SINKS>(s)) {
                             if (!mbar_wait_inline(&q_full[s], (q_par >> s) & 1u)) {
                                 if (lane == 0) report_fault(p.fault, FAULT_WAIT_Q, s);
                                 ok = false;
@@ -620,8 +627,8 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                     }
 #pragma unroll 1
                     for (int s = 0; s < 2; ++s) {
-                        if (j < pw.lo_of(s) || j >= pw.hi_of(s)) continue;
-                        if (j == pw.lo_of(s)) {
+                        if (!pw.sees<SINKS>(s, j)) continue;
+                        if (j == pw.first_of<SINKS>(s)) {
                             if (!mbar_wait_inline(&o_empty[s], (o_par >> s) & 1u)) {
                                 if (lane == 0) report_fault(p.fault, FAULT_WAIT_O, 0x100u + s);
                                 ok = false;
@@ -642,7 +649,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                             break;
                         }
                         tc_fence_after_sync();
-                        umma_ts_x4<8, 128>(tO, tP, dv, IDESC_PV, j > pw.lo_of(s) ? 1u : 0u);
+                        umma_ts_x4<8, 128>(tO, tP, dv, IDESC_PV, j > pw.first_of<SINKS>(s) ? 1u : 0u);
                         umma_ts_x2<8, 128>(tO, tP + 32, dv + 512, IDESC_PV, 1u);
                         if (!mbar_wait_inline(&p_part[2 * s + 1], par)) {
                             if (lane == 0) report_fault(p.fault, FAULT_WAIT_P, 0x1000u + r);
@@ -768,7 +775,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
             const PairWork pw = decode_pair<VISION, SINKS>(p, cur);
             if (pw.uhi == pw.ulo) continue;
             const int t = pw.q0_of(s) + r;
-            const int lo = pw.lo_of(s), hi = pw.hi_of(s);
+            const int lo = pw.lo_of(s), hi = pw.hi_of(s), first = pw.first_of<SINKS>(s);
             int row_lo = 0, row_hi = p.kv_len;  // visible keys [row_lo, row_hi)
             if (causal) {
                 const int diag = t + off;
@@ -786,8 +793,11 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
 
             float m = -CUDART_INF_F;  // running max, log2 domain, possibly stale by <= 8
             float l = 0.f;            // row sum
-            for (int j = lo; j < hi; ++j, ++g) {
-                const int kc = (SINKS ? key_block(p, j, pw.gap) : j) * C::BN;
+            int j = first;
+            if (lo == hi) j = hi;  // (nothing is seen, sinks or not)
+            for (; j < hi; ++j, ++g) {
+                if (SINKS && j == pw.gap) j = lo;
+                const int kc = (SINKS && j < pw.gap ? j - pw.ulo : j) * C::BN;
                 if (!mbar_wait_warp<3>(&s_full[s], g & 1)) {
                     report_fault(p.fault, FAULT_WAIT_S, g);
                     ok = false;
@@ -825,7 +835,7 @@ __global__ void __launch_bounds__(PairCfg::THREADS, 1)
                 }
                 tc_fence_after_sync();
                 const bool need = m_new > m + 8.0f;
-                if (j == lo) {
+                if (j == first) {
                     m = m_new;
                 } else if (__any_sync(0xffffffffu, need)) {
                     // Rare: some row's maximum grows by more than 2^8: rescale those rows of O in tensor memory.

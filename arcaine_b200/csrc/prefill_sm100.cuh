@@ -63,7 +63,7 @@ struct PrefillParams {
     const uint4* mask_bits;      // [row tile][key block][row]: one bit per key, set where the mask is 0
     int mask_blocks;
     const int* ids;  // vision-block ids, ids[j] that of key j
-    int sinks;       // the first keys that stay visible behind a window
+    int sinks, sink_blocks;  // the first keys that stay visible behind a window; their blocks
 };
 
 // A row's visible keys [lo, hi).

@@ -248,6 +248,12 @@ __device__ __forceinline__ WideWork wide_place(const PrefillParams& p, const Wid
     return t;
 }
 
+// Up to 64 sinks do not cost a whole block: of the first 64 keys, 32 of either CTA's K, scores, exponentials and sums.  It is a unit's
+// first block, and stands in front of the roles' loops.  (8192 tokens of 24/4 heads, window 1024, 186.6 -> 183.3 us; 2048 gated over
+// 5049 keys 69.4 -> 67.6.  At head dim 128, where a block is half as long and a pipeline's turn is not shorter for fewer keys,
+// such blocks brought nothing: the code that is theirs alone is fetched cold, and in the loop it was in the way.)
+__device__ __forceinline__ bool short_block(const PrefillParams& p, int j, int gap) { return j < gap && p.sinks <= 64; }
+
 template <bool MASKED, bool SPLIT, bool VISION, bool SINKS>
 __device__ __forceinline__ void wide_find_blocks(const PrefillParams& p, int rank, WideWork& t) {
     const int rows = p.head_pair ? WideCfg::BM : 2 * WideCfg::BM;  // tokens of the unit
@@ -368,7 +374,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
             if (leader && lane == 0) mbar_arrive_expect_tx(&first[c], 2 * (C::Q_CHUNK + C::K_CHUNK));
             __syncwarp();
             tma_load_4d_pair(sQ + c * C::Q_CHUNK, &tm_q, b_first + c * 8, c * 64, w.h, w.q0, w.b);
-            tma_load_4d_pair(sK + st * C::K_BYTES + c * C::K_CHUNK, &tm_k, b_first + c * 8, c * 64, w.kvh, key_of(w, w.lo) + rank * 64, w.b);
+            tma_load_4d_pair(sK + st * C::K_BYTES + c * C::K_CHUNK, &tm_k, b_first + c * 8, c * 64, w.kvh, key_of(w, w.lo) + rank * (SINKS && short_block(p, w.lo, w.gap) ? 32 : 64), w.b);
         }
     };
     auto load_k = [&](const WideWork& w, int j, int st) {
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
     } else if (warp == C::ISSUER_WARP) {
         // ------------------------------------------------------------------ MMA issuer (for both CTAs)
         if (leader) {
-            constexpr uint32_t IDESC_QK = make_idesc_bf16(256, 128, false);
+            constexpr uint32_t IDESC_QK = make_idesc_bf16(256, 128, false), IDESC_QK_SHORT = make_idesc_bf16(256, 64, false);
             constexpr uint32_t IDESC_PV = make_idesc_bf16(256, 256, true);
             const uint64_t dQ = make_smem_desc_sw128(smem_u32(sQ), 16, 1024);
             const uint64_t dK = make_smem_desc_sw128(smem_u32(sK), 16, 1024);
@@ -602,8 +608,9 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                 const int st = gs & 1;
                 uint64_t da = dQ, db = dK + (uint64_t)(st * (C::K_BYTES >> 4));
                 uint32_t acc = 0u;
+                const uint32_t idesc = SINKS && short_block(p, j, w.gap) ? IDESC_QK_SHORT : IDESC_QK;
                 auto chunk = [&]() {  // 64 head-dim columns
-                    umma_pair_ss_x4<2, 2>(tmem_base + C::COL_S + st * 128, da, db, IDESC_QK, acc);
+                    umma_pair_ss_x4<2, 2>(tmem_base + C::COL_S + st * 128, da, db, idesc, acc);
                     da += C::Q_CHUNK >> 4, db += C::K_CHUNK >> 4, acc = 1u;
                 };
                 if (j == w.lo) {
@@ -682,6 +689,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                             break;
                         }
                         tc_fence_after_sync();
+                        if (SINKS && half == 1 && short_block(p, j, w.gap)) break;
                         umma_pair_ts_x4<8, 128>(tmem_base + C::COL_O, tP, dv, IDESC_PV, acc);
                     }
                     if (!ok) break;
@@ -864,7 +872,43 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
                            : 0u;
             };
             uint32_t cls = class_of(w.lo);
-            for (int j = w.lo; j < w.hi; ++j, ++g) {
+            int j = w.lo;
+            if (SINKS && short_block(p, j, w.gap)) {  // (in front of the loop, out of the way of its code)
+                const int st = g & 1;
+                const uint32_t tS = tmem_base + lane_sel + C::COL_S + st * 128;
+                if (!mbar_wait_inline(&s_full[st], (g >> 1) & 1)) {
+                    if (lane == 0) report_fault(p.fault, FAULT_WAIT_S, 0x300u + g);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+                tmem_ld32(tS, s0);
+                tmem_ld32(tS + 32, s1);
+                tmem_wait_ld();
+                mask(s0, 0);
+                mask(s1, 32);
+                float mr[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+                chunk_max(s0, mr);
+                chunk_max(s1, mr);
+                m = fmaxf(fmaxf(mr[0], mr[1]), fmaxf(mr[2], mr[3])) * sl;
+                const float nm = m == -CUDART_INF_F ? 0.f : -m;
+                uint64_t ls2[2] = {0ull, 0ull};
+                uint32_t pk[16];  // (the largest probability is one: nothing of it is rounded)
+                exp_chunk(s0, pk, ls2, sl2, pack_f32x2(nm, nm));
+                tmem_st16(tS, pk);
+                exp_chunk(s1, pk, ls2, sl2, pack_f32x2(nm, nm));
+                tmem_st16(tS + 16, pk);
+                float l0, l1, l2, l3;
+                unpack_f32x2(ls2[0], l0, l1);
+                unpack_f32x2(ls2[1], l2, l3);
+                l = (l0 + l1) + (l2 + l3);
+                tmem_wait_st();
+                tc_fence_before_sync();
+                mbar_arrive_remote_warp(b_half + 16 * st);
+                mbar_arrive_remote_warp(b_half + 16 * st + 8);
+                ++j, ++g;
+            }
+            for (; j < w.hi; ++j, ++g) {
                 const uint32_t next_cls = class_of(j + 1);
                 const bool by_bits = (cls & (MASK_HIDDEN | MASK_VALUES)) == MASK_HIDDEN;
                 uint4 bits = make_uint4(0u, 0u, 0u, 0u);
