@@ -247,7 +247,7 @@ struct PrefillPlan {
 };
 
 // Keys that stay visible behind a call's window.  (Without a window, or behind one that hides nothing, there is nothing to keep visible.)
-static int sinks_of(const arc_sdpa_prefill_params* p) { return p->window > 0 && p->window < p->kv_len ? p->sinks : 0; }
+static int sinks_of(const arc_sdpa_prefill_params* p) { return p->window > 0 && p->window < p->kv_len ? std::min(p->sinks, p->kv_len) : 0; }
 
 // Key blocks that token tile qt (128 rows) of a call sees, block ids apart.
 static int tile_key_blocks(const arc_sdpa_prefill_params* p, int qt) {
@@ -902,7 +902,7 @@ extern "C" const char* arc_sdpa_status_string(int status) {
         case ARC_ERR_NULL_POINTER: return "required pointer is null";
         case ARC_ERR_UNSUPPORTED_GQA: return "more than 16 query heads per KV head";
         case ARC_ERR_TOO_LARGE: return "size beyond a fixed limit";
-        case ARC_ERR_DEVICE_BAD_RANGE: return "a device-side kv_len or kv_row_offset reaches past the cache";
+        case ARC_ERR_DEVICE_BAD_RANGE: return "a device-side kv_len, kv_row_offset, page or slot reaches past the cache";
         default: return "unknown status";
     }
 }

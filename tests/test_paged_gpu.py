@@ -362,7 +362,9 @@ def test_decode_edges(nq, nkv, hd, page, window, sinks, ctas):
 @pytest.mark.parametrize("lens,page,nq,nkv,hd,window,sinks,ctas", [
     ([5000], 16, 24, 4, 256, None, 0, 0), ([70001, 3], 64, 16, 2, 128, None, 0, 0), ([9000] * 40, 32, 28, 4, 128, 1024, 4, 0), ([513], 16, 8, 8, 128, None, 0, 0),
     ([800, 7, 2000, 0, 31], 16, 8, 2, 256, None, 0, 1), ([800, 7, 2000, 0, 31], 16, 8, 4, 128, 500, 20, 3), ([3000, 100], 48, 32, 16, 128, None, 0, 1000),
-    ([1] * 2000, 16, 4, 4, 128, None, 0, 0), ([300] * 129, 128, 16, 1, 256, 64, 1, 0), ([0, 0, 0], 16, 8, 4, 128, None, 0, 0)])
+    ([1] * 2000, 16, 4, 4, 128, None, 0, 0), ([300] * 129, 128, 16, 1, 256, 64, 1, 0), ([0, 0, 0], 16, 8, 4, 128, None, 0, 0),
+    ([0, 0, 0], 16, 8, 4, 128, None, 0, 7), ([5000, 4000, 17], 16, 8, 4, 256, 4090, 2**31 - 1, 0), ([5000, 4000, 17], 32, 16, 2, 128, 2**31 - 2, 9, 0),
+    ([4096] * 9, 16, 4, 2, 128, None, 0, 1), ([257] * 700, 16, 8, 1, 256, None, 0, 0)])
 def test_decode_sizes(lens, page, nq, nkv, hd, window, sinks, ctas):
     from arcaine_b200 import ops
     q, kp, vp, table, _ = paged_case(lens, page, nq, nkv, hd, window, sinks, seed=len(lens))

@@ -54,7 +54,9 @@ CASES = [  # batch, seq, kv, nq, nkv, hd, window, sinks, splits
     (1, 1, 1, 4, 2, 256, 1, 1, 0), (1, 33, 900, 8, 4, 256, 50, 4, 0), (2, 300, 300, 16, 8, 256, 64, 4, 0), (1, 260, 700, 5, 5, 256, 150, 20, 0),
     (1, 128, 3000, 8, 8, 256, 1000, 140, 0), (1, 128, 3000, 8, 8, 256, 1000, 140, 2), (1, 100, 3000, 4, 2, 256, 900, 300, 3), (1, 100, 3000, 4, 2, 256, 900, 300, 4),
     (1, 100, 3000, 4, 2, 256, 900, 300, 6), (1, 2000, 2500, 24, 4, 256, 512, 64, 0), (4, 900, 900, 16, 8, 256, 256, 8, 0), (1, 2600, 2600, 9, 3, 256, 100, 600, 0),
-    (1, 200, 150, 4, 2, 256, 30, 5, 0), (1, 384, 384, 8, 4, 256, 1, 2, 0)]
+    (1, 200, 150, 4, 2, 256, 30, 5, 0), (1, 384, 384, 8, 4, 256, 1, 2, 0),
+    (1, 500, 900, 8, 4, 128, 100, 2**31 - 1, 0), (1, 2100, 2100, 28, 4, 128, 300, 2**31 - 1, 0), (1, 500, 900, 8, 4, 256, 100, 2**31 - 1, 0),
+    (1, 300, 900, 8, 4, 256, 200, 65, 0), (1, 300, 900, 8, 4, 256, 200, 63, 0), (1, 700, 1500, 9, 3, 256, 128, 1, 0)]
 
 
 @pytest.mark.parametrize("batch,seq,kv,nq,nkv,hd,window,sinks,splits", CASES)
