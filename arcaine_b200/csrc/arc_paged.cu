@@ -190,19 +190,20 @@ static int paged_slices(int hd, int heads) { return std::max(1, std::min(64 * 10
 
 // One launch or two?  Clusters take 4.8 us and the longer of two times: of a CTA of the longest sequence, which streams 65 / 70 / 85 GB/s with
 // one / two / four and more KV heads of 128 and 91 with heads of 256, and of all keys at 6.5 TB/s.  Shares read those at the same
-// rate, whatever the lengths, but cost 6.5 us and 0.03 for each sequence (the second launch, the records, shares that two
-// sequences divide).  (us, shares and clusters, all sequences as long: one token of 24/4 heads of 256 over 513 keys 7.2 and 6.2, of
-// 28/4 of 128 over 4100 11.0 and 9.8; 16 over 1028 15.5 and 11.5; 48 26.9 and 22.2; 100 43.2 and 39.2; 128 of 16/2 over 4100
-// 94 and 83.)  Lengths on the device are not known here, only what a table row can name and what a window leaves of it.  Behind a
-// window that is shorter than that, streams tend to its length; otherwise one sequence may be as long as the table says and work
-// alone in its cluster, so the form is taken where that costs at most 20 us or 1.3 times what shares do.
+// rate, whatever the lengths, but cost 7 us, up to 3 more that parts of a few slices do not hide, and 0.03 for each sequence (the
+// second launch, the records, shares that two sequences divide).  (us, shares and clusters, all sequences as long: one token of 24/4
+// heads of 256 over 513 keys 7.2 and 6.1, of 28/4 of 128 over 4100 10.6 and 9.2; 16 over 1028 15.5 and 11.1; 48 26.9 and 22.2; 100
+// 43.2 and 39.2; 128 of 16/2 over 4100 94 and 83.)  Lengths on the device are not known here, only what a table row can name and what
+// a window leaves of it.  Behind a window that is shorter than that, streams tend to its length; otherwise one sequence may be as
+// long as the table says and work alone in its cluster, so the form is taken where that costs at most 24 us or 1.3 times what
+// shares do.
 static bool worth_cluster(const arc_sdpa_decode_paged_params* p, int heads, int size) {
     const int64_t longest = p->kv_len ? (int64_t)p->table_width * p->page_size : p->kv_len_uniform;
     const double keys = 16.0 * (double)most_slices_seen(p, longest), key = 4.0 * p->nkv * p->hd;  // bytes of one
     const double rate = p->hd == 256 ? 91e3 : heads == 1 ? 65e3 : heads < 4 ? 70e3 : 85e3;       // bytes a us
     const double alone = 4.8 + keys * key * heads / p->nkv / size / rate;
-    const auto shares = [&](double k) { return 6.5 + 0.03 * p->batch + k * key / 6.5e6; };
-    if (p->kv_len && p->batch > 1 && p->window >= longest) return alone <= std::max(20.0, 1.3 * shares(keys));
+    const auto shares = [&](double k) { return 7.0 + 3.0 * std::min(1.0, k * key / 8e6) + 0.03 * p->batch + k * key / 6.5e6; };
+    if (p->kv_len && p->batch > 1 && p->window >= longest) return alone <= std::max(24.0, 1.3 * shares(keys));
     return std::max(alone, 4.8 + keys * p->batch * key / 6.5e6) <= shares(keys * p->batch);
 }
 

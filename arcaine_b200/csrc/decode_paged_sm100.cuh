@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(288, 1)
 // Each folds its warps' records and sends them, as they are, to the CTAs that finish the columns (the largest power of two of
 // the cluster's), which weight, gate and store them: no records in global memory, no merge.  The sends are st.async, counted by
 // an mbarrier of the CTA they go to, as in decode_sm100.cuh, whose comments have what was measured against a barrier of the
-// cluster.  Length and first pages are two trips in front of the first copy.
+// cluster.
 template <int HD, int NT>
 __global__ void __launch_bounds__(288, 1)
     sdpa_decode_paged_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -504,36 +504,42 @@ __global__ void __launch_bounds__(288, 1)
     grid_launch_dependents();
     const uint32_t fault = threadIdx.x == 0 ? *reinterpret_cast<volatile uint32_t*>(p.fault) : 0u;
     const int len = p.kv_len ? p.kv_len[b] : p.kv_len_uniform;
+    // The first steps of the CTAs come in order, so that without a window a CTA's first pages, which do not depend on the length, are
+    // looked up beside it; what is left behind them is divided evenly.
+    int page = 0, row = 0;  // producer: of this lane's slice of the next step
+    auto look_up = [&](int slice) {
+        const int column = slice * 16 / p.page;
+        row = slice * 16 - column * p.page;
+        page = p.table[b * p.table_stride + column];
+    };
+    const bool early = p.window >= p.max_len;
+    if (early && warp == ncw && lane < p.slices && (rank * p.slices + lane) * 16 < p.max_len) look_up(rank * p.slices + lane);
     if (len > p.max_len) {  // (the same in all of the cluster's CTAs)
         if (threadIdx.x == 0) report_fault(p.fault, FAULT_BAD_KV_RANGE, (uint32_t)b);
         return;
     }
     const SeenKeys seen = seen_of(len, p.window, p.sinks);
-    // This CTA's slices [first, first + mine): whole steps as long as there are any.
-    const int steps_all = (seen.n + p.slices - 1) / p.slices, step0 = (int)((long long)steps_all * rank / p.ncta), step1 = (int)((long long)steps_all * (rank + 1) / p.ncta);
-    const int first = step0 * p.slices, mine = min(seen.n, step1 * p.slices) - first;
+    const int steps_all = (seen.n + p.slices - 1) / p.slices, rest = max(0, steps_all - p.ncta);
+    const int more0 = p.ncta + rest * rank / p.ncta, steps = rank < steps_all ? 1 + p.ncta + rest * (rank + 1) / p.ncta - more0 : 0;
+    auto first_of = [&](int step) { return (step == 0 ? rank : more0 + step - 1) * p.slices; };  // first slice of this CTA's step
 
     if (warp == ncw) {
         // ------------------------------------------------------------------ producer
-        const int i = lane;
-        int page = 0, row = 0;
-        auto look_up = [&](int k0) {  // of this lane's slice of the step at k0
-            if (k0 + i >= mine || i >= p.slices) return;
-            const int key = seen.slice(first + k0 + i) * 16, column = key / p.page;
-            row = key - column * p.page;
-            page = p.table[b * p.table_stride + column];
+        auto look_up_step = [&](int step) {
+            const int at = first_of(step) + lane;
+            if (step < steps && lane < p.slices && at < seen.n) look_up(seen.slice(at));
         };
-        look_up(0);
+        if (!early) look_up_step(0);
         int it = 0;
-        for (int k0 = 0; k0 < mine; k0 += p.slices, ++it) {
-            const int own_page = page, own_row = row;
-            look_up(k0 + p.slices);
+        for (; it < steps; ++it) {
+            const int own_page = page, own_row = row, n = min(p.slices, seen.n - first_of(it));
+            look_up_step(it + 1);
             const int st = it % p.stages;
             if (it >= p.stages && !mbar_wait_warp(&ring.empty[st], ((it / p.stages) - 1) & 1)) {
                 if (lane == 0) report_fault(p.fault, FAULT_WAIT_EMPTY, it);
                 break;
             }
-            ask_slices(ring, tm_k, tm_v, p, st, min(p.slices, mine - k0), own_page, own_row, head0, b);
+            ask_slices(ring, tm_k, tm_v, p, st, n, own_page, own_row, head0, b);
         }
         drain(ring, it);
     } else if (warp < ncw) {
@@ -542,17 +548,16 @@ __global__ void __launch_bounds__(288, 1)
         GroupState<HD, NT> group;
         group.load(p.q + b * p.q_stride_b + (long long)kvh * G * HD, G);
         bool ok = true;
-        int it = 0;
-        for (int k0 = 0; k0 < mine; k0 += p.slices, ++it) {
-            const int st = it % p.stages;
+        for (int it = 0; it < steps; ++it) {
+            const int st = it % p.stages, at = first_of(it) + slice;
             if (!mbar_wait_warp(&ring.full[st], (it / p.stages) & 1)) {
                 if (lane == 0) report_fault(p.fault, FAULT_WAIT_FULL, it);
                 ok = false;
                 break;
             }
-            if (k0 + slice < mine)
+            if (at < seen.n)
                 attend_slice<HD, NT>(group, smem_u32(ring.slice(st, 0, slice)) + hl * HEAD, smem_u32(ring.slice(st, 1, slice)) + hl * HEAD,
-                                     seen.keys_of(seen.slice(first + k0 + slice)), p.scale_log2);
+                                     seen.keys_of(seen.slice(at)), p.scale_log2);
             __syncwarp();
             if (lane == 0) mbar_arrive(&ring.empty[st]);
         }

@@ -201,6 +201,8 @@ __device__ __forceinline__ PairWork decode_pair(const PrefillParams& p, const Ti
     if constexpr (SINKS) {
         t.gap = t.ulo;
         t.ulo = sinks_begin(p, t.gap);
+        // (Sinks that reach into the first tile's window: the second tile's own may begin behind them.)
+        if (p.sink_blocks > t.gap) t.lo[1] = min(t.lo[1], t.gap);
     }
     return t;
 }

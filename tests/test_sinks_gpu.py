@@ -3,9 +3,14 @@
 Tolerance: bf16 roundings of the probabilities (2^-8 of sum p |v|) and of the result (2^-8 of it), and 2^-9 of sum p |v| for the fp32 sums, scores and
 rescales in between."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
+
+from helpers import ROOT
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -56,11 +61,15 @@ CASES = [  # batch, seq, kv, nq, nkv, hd, window, sinks, splits
     (1, 100, 3000, 4, 2, 256, 900, 300, 6), (1, 2000, 2500, 24, 4, 256, 512, 64, 0), (4, 900, 900, 16, 8, 256, 256, 8, 0), (1, 2600, 2600, 9, 3, 256, 100, 600, 0),
     (1, 200, 150, 4, 2, 256, 30, 5, 0), (1, 384, 384, 8, 4, 256, 1, 2, 0),
     (1, 500, 900, 8, 4, 128, 100, 2**31 - 1, 0), (1, 2100, 2100, 28, 4, 128, 300, 2**31 - 1, 0), (1, 500, 900, 8, 4, 256, 100, 2**31 - 1, 0),
-    (1, 300, 900, 8, 4, 256, 200, 65, 0), (1, 300, 900, 8, 4, 256, 200, 63, 0), (1, 700, 1500, 9, 3, 256, 128, 1, 0)]
+    (2, 1499, 1499, 28, 4, 128, 490, 64, 0), (1, 300, 900, 8, 4, 256, 200, 65, 0), (1, 300, 900, 8, 4, 256, 200, 63, 0), (1, 700, 1500, 9, 3, 256, 128, 1, 0)]
 
 
 @pytest.mark.parametrize("batch,seq,kv,nq,nkv,hd,window,sinks,splits", CASES)
 def test_sinks(batch, seq, kv, nq, nkv, hd, window, sinks, splits):
+    one_call(batch, seq, kv, nq, nkv, hd, window, sinks, splits)
+
+
+def one_call(batch, seq, kv, nq, nkv, hd, window, sinks, splits):
     from arcaine_b200 import ops
     ops.clear_device_status()
     q, k, v, gate = inputs(batch, seq, kv, nq, nkv, hd, seed=seq + kv)
@@ -115,6 +124,26 @@ def test_sinks_strides_copies_and_aliases(hd, seq):
     assert torch.equal(copy, out)
     ops.sdpa_prefill(q, k, v, out=q, **kw)
     assert torch.equal(q, out) and ops.device_status() == (0, 0)
+
+
+FORCED = r"""
+import sys
+sys.path.insert(0, sys.argv[1] + '/tests')
+import test_sinks_gpu as t
+from helpers import ROOT
+for group in ((4, 2), (3, 1), (5, 5), (8, 1)):  # two heads of a group on one tile of tokens, or two tiles of one head
+    for seq, kv in ((1, 300), (129, 129), (500, 500), (300, 800), (700, 650), (1300, 1300)):
+        for window, sinks in ((1, 1), (30, 4), (128, 128), (129, 200), (250, 64), (300, 600), (490, 7), (513, 260)):
+            t.one_call(1, seq, kv, *group, 128, window, sinks, 1)
+"""
+
+
+@pytest.mark.parametrize("kernel", ["pair", "single"])
+def test_both_kernels_of_head_dim_128(kernel):
+    """The library chooses between them by size; here each takes all calls, in a process of its own (the choice is read once)."""
+    env = dict(os.environ, ARC_SDPA_PREFILL_KERNEL=kernel, PYTHONPATH=ROOT)
+    done = subprocess.run([sys.executable, "-c", FORCED, ROOT], env=env, capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_sinks_refusals():
