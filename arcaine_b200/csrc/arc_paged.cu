@@ -164,7 +164,7 @@ extern "C" int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void
 // Decode
 // ---------------------------------------------------------------------------
 struct DecodePagedPlan {
-    int nkv_cta = 1, groups = 1, slices = 1, stages = 2, ncta = 1, nt = 1, smem_bytes = 0;
+    int nkv_cta = 1, groups = 1, subs = 1, slices = 1, stages = 2, ncta = 1, smem_bytes = 0;
     long long parts = 0;
     size_t ws_bytes = 0;
     bool cluster = false;  // one launch: `ncta` CTAs of a cluster per sequence and group of heads
@@ -178,15 +178,15 @@ static long long most_slices_seen(const arc_sdpa_decode_paged_params* p, int64_t
 
 // Stages of 16-key slices of `heads` KV heads, `slices` each; extra: bytes behind them.  False: not even two fit.
 static bool size_paged_cta(int hd, int heads, int slices, int extra, int smem_optin, DecodePagedPlan* plan) {
-    const int stage = 64 * slices * heads * hd, fixed = 1024 + 4 * 16 + extra;
+    const int stage = 64 * slices * heads * hd, fixed = 1024 + 6 * 16 + extra;
     plan->nkv_cta = heads;
     plan->slices = slices;
-    plan->stages = std::min(4, (smem_optin - kDecodeStaticSmem - fixed) / stage);
+    plan->stages = std::min(6, (smem_optin - kDecodeStaticSmem - fixed) / stage);
     plan->smem_bytes = plan->stages * stage + fixed;
     return plan->stages >= 2;
 }
 
-static int paged_slices(int hd, int heads) { return std::max(1, std::min(64 * 1024 / (64 * heads * hd), 8 / heads)); }
+static int paged_slices(int hd, int heads, int subs) { return std::max(1, std::min(64 * 1024 / (64 * heads * hd), 8 / (heads * subs))); }
 
 // One launch or two?  Clusters take 4.8 us and the longer of two times: of a CTA of the longest sequence, which streams 65 / 70 / 85 GB/s with
 // one / two / four and more KV heads of 128 and 91 with heads of 256, and of all keys at 6.5 TB/s.  Shares read those at the same
@@ -222,7 +222,7 @@ static void plan_paged_cluster(const arc_sdpa_decode_paged_params* p, const Host
     int finishers = 1;
     while (finishers * 2 <= size) finishers *= 2;
     const int extra = 64 + 8 * ((rows + 1) & ~1) * 8 + size * rows * (p->hd / finishers) * 4 + rows * 32;
-    if (!size_paged_cta(p->hd, heads, paged_slices(p->hd, heads), extra, hs.smem_optin, &one)) return;
+    if (!size_paged_cta(p->hd, heads, paged_slices(p->hd, heads, plan->subs), extra, hs.smem_optin, &one)) return;
     one.cluster = true;
     one.groups = p->nkv / heads;
     one.ncta = size;
@@ -243,12 +243,12 @@ static int plan_decode_paged(const arc_sdpa_decode_paged_params* p, const HostSt
     if (!p->kv_len && (p->kv_len_uniform < 0 || p->kv_len_uniform > (int64_t)p->table_width * p->page_size)) return ARC_ERR_BAD_SHAPE;
     const int G = p->nq / p->nkv;
     if (G > 16) return ARC_ERR_UNSUPPORTED_GQA;
-    plan->nt = G > 8 ? 2 : 1;
+    plan->subs = G > 8 ? 2 : 1;
     // KV heads of a CTA: the largest divisor of nkv whose rows are at most 2 KB; slices of a stage: 64 KB of K and V, eight warps.
     int heads = 1;
-    for (int c = 1; c <= p->nkv && c <= 1024 / p->hd; ++c)
+    for (int c = 1; c <= p->nkv && c <= 1024 / p->hd && c * plan->subs <= 8; ++c)
         if (p->nkv % c == 0) heads = c;
-    if (!size_paged_cta(p->hd, heads, paged_slices(p->hd, heads), (p->batch + 2) * 8, hs.smem_optin, plan)) return ARC_ERR_TOO_LARGE;
+    if (!size_paged_cta(p->hd, heads, paged_slices(p->hd, heads, plan->subs), (p->batch + 2) * 8, hs.smem_optin, plan)) return ARC_ERR_TOO_LARGE;
     plan->groups = p->nkv / plan->nkv_cta;
     plan->ncta = std::min(1024, std::max(1, p->num_ctas > 0 ? p->num_ctas : hs.sm_count / plan->groups));
     plan->parts = ((long long)plan->ncta + p->batch) * plan->slices;
@@ -271,14 +271,10 @@ static int allow_shared_memory(const HostState& hs) {
     static std::atomic<bool> done[kMaxDevices];
     if (done[hs.device].load(std::memory_order_acquire)) return ARC_OK;
     const int most = hs.smem_optin - kDecodeStaticSmem;
-    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<128, 1>, most));
-    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<128, 2>, most));
-    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<256, 1>, most));
-    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<256, 2>, most));
-    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<128, 1>, most));
-    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<128, 2>, most));
-    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<256, 1>, most));
-    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<256, 2>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<128>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_kernel<256>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<128>, most));
+    ARC_CUDA(opt_in_smem(sdpa_decode_paged_cluster_kernel<256>, most));
     done[hs.device].store(true, std::memory_order_release);
     return ARC_OK;
 }
@@ -310,23 +306,23 @@ static int launch_decode_paged(const arc_sdpa_decode_paged_params* p, const Deco
     kp.table_stride = p->table_stride;
     kp.scale_log2 = p->scale * 1.4426950408889634f;
     kp.nkv_cta = plan.nkv_cta;
+    kp.subs = plan.subs;
     kp.slices = plan.slices;
     kp.stages = plan.stages;
     kp.ncta = plan.ncta;
+    const unsigned threads = 32u * (unsigned)(plan.nkv_cta * plan.subs * plan.slices + 1);
     if (plan.cluster) {
         kp.gate = static_cast<const uint16_t*>(p->gate);
         kp.out = static_cast<uint16_t*>(p->out);
         kp.out_f32 = p->out_f32;
         kp.out_lse = p->out_lse;
         kp.o_stride_b = p->o_stride_b;
-        const auto kernel = plan.nt == 1 ? sdpa_decode_paged_cluster_kernel<HD, 1> : sdpa_decode_paged_cluster_kernel<HD, 2>;
-        ARC_CUDA(launch_dependent(kernel, dim3((unsigned)plan.ncta, (unsigned)plan.groups, (unsigned)p->batch), dim3(32u * (unsigned)(plan.nkv_cta * plan.slices + 1)),
+        ARC_CUDA(launch_dependent(sdpa_decode_paged_cluster_kernel<HD>, dim3((unsigned)plan.ncta, (unsigned)plan.groups, (unsigned)p->batch), dim3(threads),
                                   (size_t)plan.smem_bytes, stream, plan.ncta, tk, tv, kp));
         count_launch();
         return ARC_OK;
     }
-    const auto kernel = plan.nt == 1 ? sdpa_decode_paged_kernel<HD, 1> : sdpa_decode_paged_kernel<HD, 2>;
-    ARC_CUDA(launch_dependent(kernel, dim3((unsigned)plan.ncta, (unsigned)plan.groups), dim3(32u * (unsigned)(plan.nkv_cta * plan.slices + 1)),
+    ARC_CUDA(launch_dependent(sdpa_decode_paged_kernel<HD>, dim3((unsigned)plan.ncta, (unsigned)plan.groups), dim3(threads),
                               (size_t)plan.smem_bytes, stream, 1, tk, tv, kp));
     count_launch();
 

@@ -31,7 +31,8 @@ struct DecodePagedParams {
     long long q_stride_b, table_stride;
     float scale_log2;
     int nkv_cta;  // KV heads of a CTA (grid.y = nkv / nkv_cta)
-    int slices;   // 16-key slices of a stage; consumer warps = nkv_cta * slices
+    int subs;     // warps that divide a KV head's query heads, eight each
+    int slices;   // 16-key slices of a stage; consumer warps = nkv_cta * subs * slices
     int stages;
     int ncta;     // grid.x
     // One launch (sdpa_decode_paged_cluster_kernel): the results
@@ -42,35 +43,33 @@ struct DecodePagedParams {
     long long o_stride_b;
 };
 
-// What a consumer warp holds of its KV head's group of query heads: Q^T fragments (B operand, hd x 8 heads), running maximum (log2
-// domain) and sum, O^T.
-template <int HD, int NT>
+// What a consumer warp holds of up to eight query heads of a KV head: Q^T fragments (B operand, hd x 8 heads), running maximum (log2
+// domain) and sum, O^T.  Larger groups go to two warps, which read the same keys out of shared memory.  (Sixteen heads in one warp are
+// 192 registers at head dim 256, and spilled: us, 64 sequences of 4100 keys of 16/1 heads 84.6 -> 53.6, one of 513 11.5 -> 7.3.  At head
+// dim 128 200 of 300 27.7 -> 22.6, one of 513 5.9 -> 5.5, but 64 of 4100 27.0 -> 31.1: eight warps then have four slices a step.)
+template <int HD>
 struct GroupState {
-    uint32_t q[NT][HD / 16][2];
-    float m[NT][2], l[NT][2], o[NT][HD / 16][4];
+    uint32_t q[HD / 16][2];
+    float m[2], l[2], o[HD / 16][4];
 
-    __device__ __forceinline__ void load(const uint16_t* heads, int G) {  // heads: the group's first query head
-        const int lane = threadIdx.x & 31;
+    __device__ __forceinline__ void load(const uint16_t* heads, int G) {  // heads: the first of the G query heads
+        const int lane = threadIdx.x & 31, n = lane >> 2;
+        const bool valid = n < G;
+        const uint16_t* src = heads + (valid ? n : 0) * HD + (lane & 3) * 2;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int n = nt * 8 + (lane >> 2);
-            const bool valid = n < G;
-            const uint16_t* src = heads + (valid ? n : 0) * HD + (lane & 3) * 2;
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-                q[nt][kk][0] = valid ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
-                q[nt][kk][1] = valid ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
-            }
-            m[nt][0] = m[nt][1] = -CUDART_INF_F;
-            l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-            for (int mt = 0; mt < HD / 16; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
+        for (int kk = 0; kk < HD / 16; ++kk) {
+            q[kk][0] = valid ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
+            q[kk][1] = valid ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
         }
+        m[0] = m[1] = -CUDART_INF_F;
+        l[0] = l[1] = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < HD / 16; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
     }
 
-    // Sum of head nt * 8 + (lane & 3) * 2 + u over the key rows.
-    __device__ __forceinline__ float sum(int nt, int u) const {
-        float ls = l[nt][u];
+    // Sum of head (lane & 3) * 2 + u over the key rows.
+    __device__ __forceinline__ float sum(int u) const {
+        float ls = l[u];
         ls += __shfl_xor_sync(0xffffffffu, ls, 4);
         ls += __shfl_xor_sync(0xffffffffu, ls, 8);
         ls += __shfl_xor_sync(0xffffffffu, ls, 16);
@@ -81,8 +80,8 @@ struct GroupState {
 constexpr int SLICE_CHUNK = 16 * 128;  // 64 columns of a slice in shared memory: 16 rows x 128 bytes
 
 // One slice: sK, sV its head's rows in shared memory ([64-column chunk][row], 128-byte swizzle), bit k of vis: key k is seen.
-template <int HD, int NT>
-__device__ __forceinline__ void attend_slice(GroupState<HD, NT>& g, uint32_t sK, uint32_t sV, uint32_t vis, float sl) {
+template <int HD>
+__device__ __forceinline__ void attend_slice(GroupState<HD>& g, uint32_t sK, uint32_t sV, uint32_t vis, float sl) {
     constexpr int CHUNK = SLICE_CHUNK;
     const int lane = threadIdx.x & 31, g4 = lane >> 2;  // g4: accumulator row group
     // Swizzled addressing: 16-byte unit u of row r sits at unit u ^ (r & 7).
@@ -103,8 +102,7 @@ __device__ __forceinline__ void attend_slice(GroupState<HD, NT>& g, uint32_t sK,
         __syncwarp();
     }
     // Fragments are fetched AHEAD at a time and a batch before their MMAs (decode_sm100.cuh).
-    constexpr int AHEAD = HD * NT > 256 ? 2 : 4, BATCHES = HD / 16 / AHEAD;
-    constexpr int CHAINS = NT == 1 ? 4 : 2;  // independent sums of S
+    constexpr int AHEAD = 4, BATCHES = HD / 16 / AHEAD, CHAINS = 4;  // CHAINS: independent sums of S
     uint32_t fr[2][AHEAD][4];
     auto fetch_k = [&](int bt) {
 #pragma unroll
@@ -120,76 +118,60 @@ __device__ __forceinline__ void attend_slice(GroupState<HD, NT>& g, uint32_t sK,
             ldmatrix_x4_trans(fr[bt & 1][e], a_v + (mt >> 2) * CHUNK + ((((mt & 3) * 2 + hv) ^ xv) << 4));
         }
     };
-    float acc[NT][CHAINS][4];
+    float acc[CHAINS][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int hh = 0; hh < CHAINS; ++hh) acc[nt][hh][0] = acc[nt][hh][1] = acc[nt][hh][2] = acc[nt][hh][3] = 0.f;
+    for (int c = 0; c < CHAINS; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
     fetch_k(0);
 #pragma unroll
     for (int bt = 0; bt < BATCHES; ++bt) {
         if (bt + 1 < BATCHES) fetch_k(bt + 1);
-        else if (NT == 1) fetch_v(0);  // (an even number of batches: into the other half)
+        else fetch_v(0);  // (an even number of batches: into the other half)
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e) {
             const int kk = bt * AHEAD + e;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(acc[nt][kk % CHAINS], fr[bt & 1][e], g.q[nt][kk][0], g.q[nt][kk][1]);
+            mma_bf16_16816(acc[kk % CHAINS], fr[bt & 1][e], g.q[kk][0], g.q[kk][1]);
         }
     }
     static_assert(BATCHES % 2 == 0, "the first batch of V goes where the last one of K is not");
     const bool v_lo = (vis >> g4) & 1u, v_hi = (vis >> (g4 + 8)) & 1u;
-    uint32_t pb[NT][2];
-    bool any_rescale = false;
-    float alpha[NT][2];
+    float x[4], pr[4], alpha[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float s = acc[nt][0][e] + acc[nt][1][e];
-            if constexpr (CHAINS == 4) s += acc[nt][2][e] + acc[nt][3][e];
-            s *= sl;
-            x[e] = ((e < 2) ? v_lo : v_hi) ? s : -CUDART_INF_F;
-        }
-        float pr[4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float mx = fmaxf(x[u], x[u + 2]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float m_new = fmaxf(g.m[nt][u], mx);
-            const float m_eff = (m_new == -CUDART_INF_F) ? 0.f : m_new;
-            alpha[nt][u] = (m_new == -CUDART_INF_F) ? 1.f : fast_exp2(g.m[nt][u] - m_new);
-            pr[u] = fast_exp2(x[u] - m_eff);
-            pr[u + 2] = fast_exp2(x[u + 2] - m_eff);
-            g.l[nt][u] = g.l[nt][u] * alpha[nt][u] + pr[u] + pr[u + 2];
-            g.m[nt][u] = m_new;
-            any_rescale |= alpha[nt][u] != 1.f;
-        }
-        pb[nt][0] = movmatrix_trans(pack_bf16x2(pr[0], pr[1]));
-        pb[nt][1] = movmatrix_trans(pack_bf16x2(pr[2], pr[3]));
+    for (int e = 0; e < 4; ++e) {
+        const float s = ((acc[0][e] + acc[1][e]) + (acc[2][e] + acc[3][e])) * sl;
+        x[e] = ((e < 2) ? v_lo : v_hi) ? s : -CUDART_INF_F;
     }
+    bool any_rescale = false;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        float mx = fmaxf(x[u], x[u + 2]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float m_new = fmaxf(g.m[u], mx);
+        const float m_eff = (m_new == -CUDART_INF_F) ? 0.f : m_new;
+        alpha[u] = (m_new == -CUDART_INF_F) ? 1.f : fast_exp2(g.m[u] - m_new);
+        pr[u] = fast_exp2(x[u] - m_eff);
+        pr[u + 2] = fast_exp2(x[u + 2] - m_eff);
+        g.l[u] = g.l[u] * alpha[u] + pr[u] + pr[u + 2];
+        g.m[u] = m_new;
+        any_rescale |= alpha[u] != 1.f;
+    }
+    // (Probabilities as bf16 for the second MMA, 2^-8 of each at most; their sums as they are.)
+    const uint32_t pb[2] = {movmatrix_trans(pack_bf16x2(pr[0], pr[1])), movmatrix_trans(pack_bf16x2(pr[2], pr[3]))};
     if (__any_sync(0xffffffffu, any_rescale)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int mt = 0; mt < HD / 16; ++mt) {
-                g.o[nt][mt][0] *= alpha[nt][0];
-                g.o[nt][mt][1] *= alpha[nt][1];
-                g.o[nt][mt][2] *= alpha[nt][0];
-                g.o[nt][mt][3] *= alpha[nt][1];
-            }
+        for (int mt = 0; mt < HD / 16; ++mt) {
+            g.o[mt][0] *= alpha[0];
+            g.o[mt][1] *= alpha[1];
+            g.o[mt][2] *= alpha[0];
+            g.o[mt][3] *= alpha[1];
+        }
     }
-    if (NT > 1) fetch_v(0);
 #pragma unroll
     for (int bt = 0; bt < BATCHES; ++bt) {
         if (bt + 1 < BATCHES) fetch_v(bt + 1);
 #pragma unroll
-        for (int e = 0; e < AHEAD; ++e)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(g.o[nt][bt * AHEAD + e], fr[bt & 1][e], pb[nt][0], pb[nt][1]);
+        for (int e = 0; e < AHEAD; ++e) mma_bf16_16816(g.o[bt * AHEAD + e], fr[bt & 1][e], pb[0], pb[1]);
     }
 }
 
@@ -228,39 +210,37 @@ __device__ __forceinline__ void drain(const PagedRing& r, int it) {
     }
 }
 
-// Folds the records of a CTA's consumer warps, of which `slices` share a KV head (hl: this warp's, slice: its place among them), through the
-// shared memory at `smem`, which nothing else uses any more.  weigh(n, s, mx, z, wt) gets maximum and sum over the slices of the KV head's
-// row n and this lane's slice's weight relative to the maximum, in eight lanes per row (s: slice, from `slices` on none), and
+// Folds the records of a CTA's consumer warps, of which `slices` have the same G heads (set, of `sets`: this warp's heads, slice: its place among them), through the
+// shared memory at `smem`, which nothing else uses any more.  weigh(n, s, mx, z, wt) gets maximum and sum over the slices of the set's
+// head n and this lane's slice's weight relative to the maximum, in eight lanes per row (s: slice, from `slices` on none), and
 // returns what the slice's values are multiplied by; store(n, d, sum) gets columns d to d + 3.  All of it runs once per call, from
 // instructions fetched cold, so loops are rolled and the weights worked out once.  (A row at a time, normalised records with
 // log-sum-exps: one token of 28/4 heads of 128 over 513 keys 9.3 us, of which the fold was 2.8.)
-template <int HD, int NT, typename W, typename S>
-__device__ __forceinline__ void fold_warps(const GroupState<HD, NT>& group, uint8_t* smem, int ncw, int nkv_cta, int slices, int hl, int slice, int G, W&& weigh, S&& store) {
+template <int HD, typename W, typename S>
+__device__ __forceinline__ void fold_warps(const GroupState<HD>& group, uint8_t* smem, int sets, int slices, int set, int slice, int G, W&& weigh, S&& store) {
     constexpr int RS = HD + 4;  // floats from one head's row of a warp's record to the next
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, q4 = lane & 3;
-    float* rec = reinterpret_cast<float*>(smem);                                   // [warp][NT * 8 heads][RS]
-    float2* rec_ml = reinterpret_cast<float2*>(rec + (size_t)ncw * NT * 8 * RS);  // [warp][NT * 8]
-    float* rec_w = reinterpret_cast<float*>(rec_ml + ncw * NT * 8);
-    static_assert(NT * 8 * (RS + 3) <= 2 * 16 * HD, "a warp's records, sums and weights in its slices of K and V of two stages");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, q4 = lane & 3, ncw = sets * slices;
+    float* rec = reinterpret_cast<float*>(smem);                                   // [warp][8 heads][RS]
+    float2* rec_ml = reinterpret_cast<float2*>(rec + (size_t)ncw * 8 * RS);  // [warp][8]
+    float* rec_w = reinterpret_cast<float*>(rec_ml + ncw * 8);
+    static_assert(2 * 8 * (RS + 3) <= 2 * 16 * HD, "records, sums and weights of two warps in a KV head's slice of K and V of two stages");
     consumer_sync(ncw);  // every warp is through with the stages; no copy is in flight any more
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int u = 0; u < 2; ++u) {
+        const float ls = group.sum(u);
+        const int n = warp * 8 + q4 * 2 + u;
+        if (g4 == 0) rec_ml[n] = make_float2(group.m[u], ls);
+        float* dst = rec + (size_t)n * RS + g4;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float ls = group.sum(nt, u);
-            const int n = warp * NT * 8 + nt * 8 + q4 * 2 + u;
-            if (g4 == 0) rec_ml[n] = make_float2(group.m[nt][u], ls);
-            float* dst = rec + (size_t)n * RS + g4;
-#pragma unroll
-            for (int mt = 0; mt < HD / 16; ++mt) {
-                dst[mt * 16] = group.o[nt][mt][u];
-                dst[mt * 16 + 8] = group.o[nt][mt][u + 2];
-            }
+        for (int mt = 0; mt < HD / 16; ++mt) {
+            dst[mt * 16] = group.o[mt][u];
+            dst[mt * 16 + 8] = group.o[mt][u + 2];
         }
+    }
     consumer_sync(ncw);
 #pragma unroll 1
-    for (int n0 = slice * 4; n0 < G; n0 += slices * 4) {  // four rows of the KV head a turn, a lane per slice
-        const int n = n0 + (lane >> 3), s = lane & 7, at = (s * nkv_cta + hl) * NT * 8 + n;
+    for (int n0 = slice * 4; n0 < G; n0 += slices * 4) {  // four heads a turn, a lane per slice
+        const int n = n0 + (lane >> 3), s = lane & 7, at = (s * sets + set) * 8 + n;
         const bool some = n < G && s < slices;
         const float2 ml = some ? rec_ml[at] : make_float2(-CUDART_INF_F, 0.f);
         float mx = ml.x;
@@ -278,22 +258,22 @@ __device__ __forceinline__ void fold_warps(const GroupState<HD, NT>& group, uint
 #pragma unroll 1
     for (int i = slice; i < G * (HD / 128); i += slices) {  // half a row (head dim 256) a turn
         const int n = i / (HD / 128), d = i % (HD / 128) * 128 + lane * 4;
-        const float* src = rec + (size_t)(hl * NT * 8 + n) * RS + d;
-        const float* wts = rec_w + hl * NT * 8 + n;
+        const float* src = rec + (size_t)(set * 8 + n) * RS + d;
+        const float* wts = rec_w + set * 8 + n;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
         for (int s = 0; s < slices; ++s) {
             const float wt = *wts;
             const float4 v = *reinterpret_cast<const float4*>(src);
             acc.x = fmaf(wt, v.x, acc.x), acc.y = fmaf(wt, v.y, acc.y), acc.z = fmaf(wt, v.z, acc.z), acc.w = fmaf(wt, v.w, acc.w);
-            src += (size_t)nkv_cta * NT * 8 * RS, wts += nkv_cta * NT * 8;
+            src += (size_t)sets * 8 * RS, wts += sets * 8;
         }
         store(n, d, acc);
     }
 }
 
 // Equal shares: CTA x takes slices [x * per, (x + 1) * per) of all; grid.y: groups of KV heads.
-template <int HD, int NT>
+template <int HD>
 __global__ void __launch_bounds__(288, 1)
     sdpa_decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                              const DecodePagedParams p) {
@@ -301,7 +281,7 @@ __global__ void __launch_bounds__(288, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr int HEAD = HD / 64 * SLICE_CHUNK;
 
-    const int ncw = p.nkv_cta * p.slices;  // consumer warps
+    const int sets = p.nkv_cta * p.subs, ncw = sets * p.slices;  // sets of query heads, consumer warps
     PagedRing ring;
     ring.slice_bytes = p.nkv_cta * HEAD;
     ring.tile_bytes = p.slices * ring.slice_bytes;
@@ -389,18 +369,19 @@ __global__ void __launch_bounds__(288, 1)
         drain(ring, it);
     } else if (warp < ncw) {
         // ------------------------------------------------------------------ consumers: a KV head, a slice of every step
-        const int hl = warp % p.nkv_cta, slice = warp / p.nkv_cta, kvh = head0 + hl;
+        const int set = warp % sets, slice = warp / sets, hl = set / p.subs, sub = set - hl * p.subs;
+        const int own = min(8, G - 8 * sub), own0 = (head0 + hl) * G + 8 * sub;  // this warp's query heads
         const int g4 = lane >> 2, q4 = lane & 3;  // accumulator row group, column pair
         int it = 0;
         bool ok = true;
         long long g = g0;
-        GroupState<HD, NT> group;
+        GroupState<HD> group;
         while (ok && g < g1) {
             while (cum[b + 1] <= g) ++b;
             const long long seg_end = min(g1, cum[b + 1]);
             const SeenKeys seen = seen_of(length(b), p.window, p.sinks);
             const int first = (int)(g - cum[b]), seg = (int)(seg_end - g);
-            group.load(p.q + b * p.q_stride_b + (long long)kvh * G * HD, G);
+            group.load(p.q + b * p.q_stride_b + (long long)own0 * HD, own);
             for (int k0 = 0; k0 < seg; k0 += p.slices, ++it) {
                 const int st = it % p.stages;
                 if (!mbar_wait_warp(&ring.full[st], (it / p.stages) & 1)) {
@@ -409,7 +390,7 @@ __global__ void __launch_bounds__(288, 1)
                     break;
                 }
                 if (k0 + slice < seg)
-                    attend_slice<HD, NT>(group, smem_u32(ring.slice(st, 0, slice)) + hl * HEAD, smem_u32(ring.slice(st, 1, slice)) + hl * HEAD,
+                    attend_slice<HD>(group, smem_u32(ring.slice(st, 0, slice)) + hl * HEAD, smem_u32(ring.slice(st, 1, slice)) + hl * HEAD,
                                          seen.keys_of(seen.slice(first + k0 + slice)), p.scale_log2);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ring.empty[st]);
@@ -421,31 +402,29 @@ __global__ void __launch_bounds__(288, 1)
             const long long part = ((long long)blockIdx.x + b) * p.slices;
             if (p.slices > 1 && seg_end == g1) {  // CTA-uniform
                 if (!ok) break;
-                const long long row0 = part * p.nq + (long long)kvh * G;
-                fold_warps<HD, NT>(group, smem, ncw, p.nkv_cta, p.slices, hl, slice, G,
+                const long long row0 = part * p.nq + own0;
+                fold_warps<HD>(group, smem, sets, p.slices, set, slice, own,
                     [&](int n, int s, float mx, float z, float wt) {
-                        if (n < G && s == 0) p.part_lse[row0 + n] = z == 0.f ? -CUDART_INF_F : (mx + fast_log2(z)) * 0.6931471805599453f;
+                        if (n < own && s == 0) p.part_lse[row0 + n] = z == 0.f ? -CUDART_INF_F : (mx + fast_log2(z)) * 0.6931471805599453f;
                         return z == 0.f ? 0.f : __fdividef(wt, z);
                     },
                     [&](int n, int d, float4 v) { *reinterpret_cast<float4*>(p.part_o + (row0 + n) * HD + d) = v; });
             } else if (ok) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int u = 0; u < 2; ++u) {
+                    const float ls = group.sum(u);
+                    const float inv = ls == 0.f ? 0.f : 1.f / ls;  // (what is no number goes on to the result)
+                    const int n = q4 * 2 + u;
+                    if (n >= own) continue;
+                    const long long row = (part + slice) * p.nq + own0 + n;
+                    if (g4 == 0) p.part_lse[row] = ls == 0.f ? -CUDART_INF_F : (group.m[u] + fast_log2(ls)) * 0.6931471805599453f;
+                    float* dst = p.part_o + row * HD + g4;
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float ls = group.sum(nt, u);
-                        const float inv = ls == 0.f ? 0.f : 1.f / ls;  // (what is no number goes on to the result)
-                        const int n = nt * 8 + q4 * 2 + u;
-                        if (n >= G) continue;
-                        const long long row = (part + slice) * p.nq + (long long)kvh * G + n;
-                        if (g4 == 0) p.part_lse[row] = ls == 0.f ? -CUDART_INF_F : (group.m[nt][u] + fast_log2(ls)) * 0.6931471805599453f;
-                        float* dst = p.part_o + row * HD + g4;
-#pragma unroll
-                        for (int mt = 0; mt < HD / 16; ++mt) {
-                            dst[mt * 16] = group.o[nt][mt][u] * inv;
-                            dst[mt * 16 + 8] = group.o[nt][mt][u + 2] * inv;
-                        }
+                    for (int mt = 0; mt < HD / 16; ++mt) {
+                        dst[mt * 16] = group.o[mt][u] * inv;
+                        dst[mt * 16 + 8] = group.o[mt][u + 2] * inv;
                     }
+                }
             }
             g = seg_end;
         }
@@ -460,7 +439,7 @@ __global__ void __launch_bounds__(288, 1)
 // the cluster's), which weight, gate and store them: no records in global memory, no merge.  The sends are st.async, counted by
 // an mbarrier of the CTA they go to, as in decode_sm100.cuh, whose comments have what was measured against a barrier of the
 // cluster.
-template <int HD, int NT>
+template <int HD>
 __global__ void __launch_bounds__(288, 1)
     sdpa_decode_paged_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                                      const DecodePagedParams p) {
@@ -468,7 +447,7 @@ __global__ void __launch_bounds__(288, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr int HEAD = HD / 64 * SLICE_CHUNK;
 
-    const int ncw = p.nkv_cta * p.slices;  // consumer warps
+    const int sets = p.nkv_cta * p.subs, ncw = sets * p.slices;  // sets of query heads, consumer warps
     PagedRing ring;
     ring.slice_bytes = p.nkv_cta * HEAD;
     ring.tile_bytes = p.slices * ring.slice_bytes;
@@ -549,9 +528,10 @@ __global__ void __launch_bounds__(288, 1)
         drain(ring, it);
     } else if (warp < ncw) {
         // ------------------------------------------------------------------ consumers
-        const int hl = warp % p.nkv_cta, slice = warp / p.nkv_cta, kvh = head0 + hl;
-        GroupState<HD, NT> group;
-        group.load(p.q + b * p.q_stride_b + (long long)kvh * G * HD, G);
+        const int set = warp % sets, slice = warp / sets, hl = set / p.subs, sub = set - hl * p.subs;
+        const int own = min(8, G - 8 * sub), own0 = hl * G + 8 * sub;  // this warp's query heads of the CTA's
+        GroupState<HD> group;
+        group.load(p.q + b * p.q_stride_b + (long long)(head0 * G + own0) * HD, own);
         bool ok = true;
         for (int it = 0; it < steps; ++it) {
             const int st = it % p.stages, at = first_of(it) + slice;
@@ -561,17 +541,17 @@ __global__ void __launch_bounds__(288, 1)
                 break;
             }
             if (at < seen.n)
-                attend_slice<HD, NT>(group, smem_u32(ring.slice(st, 0, slice)) + hl * HEAD, smem_u32(ring.slice(st, 1, slice)) + hl * HEAD,
+                attend_slice<HD>(group, smem_u32(ring.slice(st, 0, slice)) + hl * HEAD, smem_u32(ring.slice(st, 1, slice)) + hl * HEAD,
                                      seen.keys_of(seen.slice(at)), p.scale_log2);
             __syncwarp();
             if (lane == 0) mbar_arrive(&ring.empty[st]);
         }
         if (lane == 0 && (!ok || fault != 0u)) *reinterpret_cast<volatile int*>(gave_up) = 1;  // (no result is written)
         const uint32_t bar = smem_u32(gathered);
-        fold_warps<HD, NT>(group, smem, ncw, p.nkv_cta, p.slices, hl, slice, G,
+        fold_warps<HD>(group, smem, sets, p.slices, set, slice, own,
             [&](int n, int s, float mx, float z, float wt) {
-                if (n < G && s < finishers) {
-                    float2* to = cml + rank * rows2 + hl * G + n;
+                if (n < own && s < finishers) {
+                    float2* to = cml + rank * rows2 + own0 + n;
                     if (alone) *to = make_float2(mx, z);
                     else st_async_f32x2(map_to_cta(smem_u32(to), s), make_float2(mx, z), map_to_cta(bar, s));
                 }
@@ -580,7 +560,7 @@ __global__ void __launch_bounds__(288, 1)
                 return wt * 0.015625f;
             },
             [&](int n, int d, float4 v) {
-                float* at = crec + (size_t)(rank * rows + hl * G + n) * dc + (d & (dc - 1));
+                float* at = crec + (size_t)(rank * rows + own0 + n) * dc + (d & (dc - 1));
                 const int to = d >> dc_log2;
                 if (alone) *reinterpret_cast<float4*>(at) = v;
                 else st_async_f32x4(map_to_cta(smem_u32(at), to), v, map_to_cta(bar, to));
