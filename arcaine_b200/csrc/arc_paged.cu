@@ -178,10 +178,10 @@ static long long most_slices_seen(const arc_sdpa_decode_paged_params* p, int64_t
 
 // Stages of 16-key slices of `heads` KV heads, `slices` each; extra: bytes behind them.  False: not even two fit.
 static bool size_paged_cta(int hd, int heads, int slices, int extra, int smem_optin, DecodePagedPlan* plan) {
-    const int stage = 64 * slices * heads * hd, fixed = 1024 + 6 * 16 + extra;
+    const int stage = 64 * slices * heads * hd, fixed = 1024 + 4 * 16 + extra;
     plan->nkv_cta = heads;
     plan->slices = slices;
-    plan->stages = std::min(6, (smem_optin - kDecodeStaticSmem - fixed) / stage);
+    plan->stages = std::min(4, (smem_optin - kDecodeStaticSmem - fixed) / stage);
     plan->smem_bytes = plan->stages * stage + fixed;
     return plan->stages >= 2;
 }
