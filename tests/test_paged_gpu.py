@@ -359,6 +359,23 @@ def test_decode_edges(nq, nkv, hd, page, window, sinks, ctas):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("nq,nkv,hd", [(9, 1, 256), (16, 1, 256), (24, 2, 256), (39, 3, 256), (9, 1, 128), (60, 4, 128)])
+@pytest.mark.parametrize("ctas", [0, 148])
+@pytest.mark.parametrize("page,window,sinks", [(16, None, 0), (32, 20, 0), (64, 17, 4), (16, 33, 17)])
+def test_decode_wide_groups(nq, nkv, hd, page, window, sinks, ctas):
+    """More than eight query heads to a KV head: two warps divide them, the second with fewer heads than the first."""
+    from arcaine_b200 import ops
+    q, kp, vp, table, gate = paged_case(EDGES, page, nq, nkv, hd, window, sinks, seed=nq + page, interleave=page == 32)
+    more = dict(scale=hd ** -0.5, window=ops.NO_WINDOW if window is None else window, sinks=sinks, num_ctas=ctas)
+    want, want_lse, size = plain_decode(q, kp, vp, table, EDGES, window, sinks, hd ** -0.5)
+    out, o32, lse = ops.sdpa_decode_paged(q, kp, vp, table, ints(EDGES), return_partial=True, **more)
+    assert ops.device_status() == (0, 0)
+    assert_attention(out, lse, want, want_lse, size)
+    assert_attention(o32, None, want, want_lse, size, rounded=False)
+    want, _, size = plain_decode(q, kp, vp, table, EDGES, window, sinks, hd ** -0.5, gate)
+    assert_attention(ops.sdpa_decode_paged(q, kp, vp, table, ints(EDGES), gate=gate, **more), None, want, want_lse, size)
+
+
 @pytest.mark.parametrize("lens,page,nq,nkv,hd,window,sinks,ctas", [
     ([5000], 16, 24, 4, 256, None, 0, 0), ([70001, 3], 64, 16, 2, 128, None, 0, 0), ([9000] * 40, 32, 28, 4, 128, 1024, 4, 0), ([513], 16, 8, 8, 128, None, 0, 0),
     ([800, 7, 2000, 0, 31], 16, 8, 2, 256, None, 0, 1), ([800, 7, 2000, 0, 31], 16, 8, 4, 128, 500, 20, 3), ([3000, 100], 48, 32, 16, 128, None, 0, 1000),
