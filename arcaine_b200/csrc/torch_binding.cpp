@@ -121,6 +121,13 @@ View view_of(const Tensor& t, const char* name) {
     return v;
 }
 
+// The same with dense strides where there is no second element to be apart from: those of a transposed view may be anything.
+View settled(View v) {
+    for (int i = v.dim - 1; i >= 0; --i)
+        if (v.n[i] <= 1) v.st[i] = i == v.dim - 1 ? 1 : v.n[i + 1] * v.st[i + 1];
+    return v;
+}
+
 View unsqueeze0(const View& a) {
     View v = a;
     v.dim = a.dim + 1;
@@ -702,7 +709,7 @@ const Tensor& table_of(PyObject* o, const Tensor& ref, int64_t batch) {
 View pool_of(PyObject* o, const Tensor& ref, int64_t nkv, int64_t hd, const char* name) {
     const Tensor& t = need_tensor(o, at::kBFloat16, name);
     same_device(t, ref, name);
-    const View v = view_of(t, name);
+    const View v = settled(view_of(t, name));
     if (v.dim != 4 || v.n[2] != nkv || v.n[3] != hd) bad(std::string(name) + " must be (num_pages, page_size, nkv, head_dim)");
     if (v.st[3] != 1 || v.st[2] != hd) bad(std::string(name) + ": the (heads, head_dim) block of every row must be contiguous");
     if (v.n[0] > 0x7fffffffll || v.n[1] > 0x7fffffffll) bad(std::string(name) + " is too large");
@@ -713,7 +720,7 @@ View pool_of(PyObject* o, const Tensor& ref, int64_t nkv, int64_t hd, const char
 View rows_of(PyObject* o, const Tensor& ref, int64_t tokens, int64_t heads, int64_t hd, const char* name) {
     const Tensor& t = need_tensor(o, at::kBFloat16, name);
     same_device(t, ref, name);
-    const View v = view_of(t, name);
+    const View v = settled(view_of(t, name));
     if (v.dim != 3 || v.n[0] != tokens || (heads >= 0 && v.n[1] != heads) || v.n[2] != hd)
         bad(std::string(name) + " must be (tokens, heads, head_dim), as the rest of the call");
     if (v.st[2] != 1 || v.st[1] != hd) bad(std::string(name) + ": the (heads, head_dim) block of every token must be contiguous");
@@ -857,7 +864,7 @@ PyObject* py_decode_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     need_args(n, 16, "sdpa_decode_paged");
     const Tensor& tq = need_tensor(a[0], at::kBFloat16, "q");
-    const View q = view_of(tq, "q");
+    const View q = settled(view_of(tq, "q"));
     if (q.dim != 3) bad("q must be (B, nq, hd)");
     const int64_t B = q.n[0], nq = q.n[1], hd = q.n[2];
     if (q.st[2] != 1 || q.st[1] != hd) bad("q: (nq, hd) must be contiguous");
@@ -883,10 +890,10 @@ PyObject* py_decode_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!is_none(a[9])) {
         const Tensor& t = need_tensor(a[9], at::kBFloat16, "out");
         same_device(t, tq, "out");
-        out = view_of(t, "out");
+        out = settled(view_of(t, "out"));
     } else if (to_bool(a[11])) {
         made = new_cuda({B, nq, hd}, at::kBFloat16, tq.device());
-        out = view_of(made, "out");
+        out = settled(view_of(made, "out"));
     }
     if (out.given()) {
         if (out.dim != 3 || out.n[0] != B || out.n[1] != nq || out.n[2] != hd || out.st[2] != 1 || out.st[1] != hd)
@@ -896,7 +903,7 @@ PyObject* py_decode_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!is_none(a[8])) {
         const Tensor& t = need_tensor(a[8], at::kBFloat16, "gate");
         same_device(t, tq, "gate");
-        const View gate = view_of(t, "gate");
+        const View gate = settled(view_of(t, "gate"));
         if (!out.given() || !same_layout(gate, out)) bad("gate must be laid out like out");
         p.gate = gate.ptr;
     }

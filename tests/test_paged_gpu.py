@@ -409,6 +409,31 @@ def test_decode_length_on_the_host_and_own_buffers():
     assert ops.device_status() == (0, 0)
 
 
+def test_views_of_one_head_or_one_token():
+    """Where a dimension has one element its stride means nothing: transposed views are taken as they come."""
+    from arcaine_b200 import ops
+    positions, inv = ints([3, 4, 5]), ops.rope_frequencies(128, device=DEV)[0]
+    k = seeded_bf16(1, 3, 128, seed=1).cuda().transpose(0, 1)  # (3, 1, 128)
+    want_k = k.contiguous()
+    pool = torch.zeros(2, 1, 16, 128, dtype=torch.bfloat16, device=DEV)  # one head, in front of the rows
+    want_pool = torch.zeros(2, 16, 1, 128, dtype=torch.bfloat16, device=DEV)
+    slots = ints([17, 0, 18])
+    ops.qkv_prepare_paged(None, want_k.clone(), want_k.clone(), positions, inv, k_pages=want_pool, v_pages=want_pool.clone(), slots=slots)
+    ops.qkv_prepare_paged(None, k, k.clone(), positions, inv, k_pages=pool.transpose(1, 2), v_pages=pool.clone().transpose(1, 2), slots=slots)
+    assert torch.equal(pool.transpose(1, 2), want_pool) and bool(want_pool.any())
+    q = seeded_bf16(4, 1, 128, seed=2).cuda().transpose(0, 1)  # (1, 4, 128)
+    got, want = torch.empty_like(q), torch.empty_like(q)
+    ops.qkv_prepare_paged(q, None, None, positions[:1], inv, q_out=got)
+    ops.qkv_prepare_paged(q.clone(memory_format=torch.contiguous_format).reshape(4, 128)[None], None, None, positions[:1], inv, q_out=want)
+    assert torch.equal(got, want)
+    pages, table = seeded_bf16(2, 1, 16, 128, seed=3).cuda(), ints([[1, 0]])
+    dense = pages.transpose(1, 2).reshape(2, 16, 1, 128).clone()
+    out = torch.empty(4, 1, 128, dtype=torch.bfloat16, device=DEV).transpose(0, 1)
+    ops.sdpa_decode_paged(q, pages.transpose(1, 2), pages.transpose(1, 2), table, 20, scale=0.1, out=out)
+    want = ops.sdpa_decode_paged(q.reshape(4, 128)[None], dense, dense, table, 20, scale=0.1)
+    assert ops.device_status() == (0, 0) and torch.equal(out, want)
+
+
 def test_decode_infinite_and_missing_numbers_stay_in_their_row():
     from arcaine_b200 import ops
     lens = [700, 700, 700]
