@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(TABLES_THREADS) paged_tables_kernel(const Page
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         if (i >= per || b0 + i >= p.batch) continue;
-        const long long most = (long long)p.width * p.page;
+        const long long most = min((long long)p.width * p.page, 0x7fffffffll);  // (positions and lengths are 32 bits wide)
         if (past[i] < 0 || fresh[i] < 0 || (long long)past[i] + fresh[i] > most) {
             report_fault(p.fault, FAULT_BAD_KV_RANGE, (uint32_t)(b0 + i));
             bad = true;

@@ -327,7 +327,7 @@ int arc_qkv_prepare(const arc_qkv_prepare_params* p, void* stream);
  * b, token_begin[batch] their number; pages_used[0] = pages the step needs from the list.  Where the list is too short for that,
  * table entries and slots without a page are -1.  Entries of slots / positions behind the last token, up to num_tokens,
  * are -1 (padding that arc_qkv_prepare_paged passes over), so that a captured step may bring fewer tokens.
- * A negative length, one that does not fit the table's row, or more than num_tokens tokens: nothing is written, and
+ * A negative length, one that does not fit the table's row (or 31 bits), or more than num_tokens tokens: nothing is written, and
  * arc_sdpa_device_status() shows ARC_ERR_DEVICE_BAD_RANGE (detail: the request; batch where the sum is too large).
  * batch <= 2048.  kv_len must not overlap past_len.  4-byte alignment is enough. */
 typedef struct arc_paged_tables_params {

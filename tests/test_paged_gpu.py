@@ -98,6 +98,23 @@ def test_tables_bad_lengths_write_nothing(new, past, tokens, detail):
     ops.clear_device_status()
 
 
+def test_tables_of_lengths_about_31_bits():
+    """A row of large pages may name more keys than 32 bits count: what passes them is refused, what does not is served."""
+    from arcaine_b200 import ops
+    page, last = 2**30, 2**31 - 1
+    for past, new, fits in ((last, 2, False), (last - 1, 2, False), (2, last, False), (last - 2, 2, True), (last, 0, True)):
+        table = ints([[0, 1, -7, -7], [0, 1, -7, -7]])
+        out = tuple(torch.full((n,), 5, dtype=torch.int32, device=DEV) for n in (2, 2, 3, 2, 1))
+        ops.paged_tables(ints([0, new]), ints([7, past]), table, ints([3, 4]), page_size=page, num_tokens=2, out=out)
+        assert ops.device_status() == ((0, 0) if fits else (10, 1))
+        ops.clear_device_status()
+        if fits:
+            want = plain_tables([0, new], [7, past], [[0, 1, -7, -7]] * 2, [3, 4], page, 2)
+            assert [t.tolist() for t in out] == list(want[:5]) and table.tolist() == want[5]
+        else:
+            assert bool((table[:, 2:] == -7).all()) and all(bool((t == 5).all()) for t in out)
+
+
 def test_tables_refusals():
     from arcaine_b200 import ops
     one, table, free = ints([1, 1]), torch.zeros(2, 4, dtype=torch.int32, device=DEV), ints([1, 2, 3])
