@@ -30,7 +30,7 @@ extern "C" int arc_paged_tables(const arc_paged_tables_params* p, void* stream) 
     if (p->batch <= 0 || p->num_tokens < 0 || p->table_width < 1 || p->free_count < 0 || p->table_stride < p->table_width ||
         p->page_size < 16 || p->page_size % 16 != 0)
         return ARC_ERR_BAD_SHAPE;
-    if (p->batch > TABLES_MAX_BATCH) return ARC_ERR_TOO_LARGE;
+    if (p->batch > TABLES_MAX_BATCH || p->num_tokens > 1 << 30) return ARC_ERR_TOO_LARGE;  // (tokens are counted in 32 bits, a grid at a time)
     if (!p->new_len || !p->block_table || (p->free_count > 0 && !p->free_pages) || (p->num_tokens > 0 && (!p->slots || !p->positions)) ||
         !p->token_begin || !p->kv_len || !p->pages_used)
         return ARC_ERR_NULL_POINTER;

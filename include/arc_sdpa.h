@@ -329,7 +329,7 @@ int arc_qkv_prepare(const arc_qkv_prepare_params* p, void* stream);
  * are -1 (padding that arc_qkv_prepare_paged passes over), so that a captured step may bring fewer tokens.
  * A negative length, one that does not fit the table's row (or 31 bits), or more than num_tokens tokens: nothing is written, and
  * arc_sdpa_device_status() shows ARC_ERR_DEVICE_BAD_RANGE (detail: the request; batch where the sum is too large).
- * batch <= 2048.  kv_len must not overlap past_len.  4-byte alignment is enough. */
+ * batch <= 2048, num_tokens <= 2^30.  kv_len must not overlap past_len.  4-byte alignment is enough. */
 typedef struct arc_paged_tables_params {
     const int32_t* new_len;    /* [batch] */
     const int32_t* past_len;   /* [batch] or NULL */

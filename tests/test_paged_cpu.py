@@ -66,6 +66,7 @@ def test_tables_refusals():
                dict(free_count=-1)):
         assert call(**kw) == _lib.ARC_ERR_BAD_SHAPE, kw
     assert call(batch=2049) == _lib.ARC_ERR_TOO_LARGE
+    assert call(num_tokens=2**30 + 1) == call(num_tokens=2**31 - 1) == _lib.ARC_ERR_TOO_LARGE
     for f in ("new_len", "block_table", "free_pages", "slots", "positions", "token_begin", "kv_len", "pages_used"):
         assert call(**{f: None}) == _lib.ARC_ERR_NULL_POINTER, f
     assert call(kv_len=m.base + 2) == _lib.ARC_ERR_ALIGNMENT
