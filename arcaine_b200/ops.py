@@ -95,6 +95,7 @@ def sdpa_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: fl
     ``sinks`` (causal masks without block ids): the first keys stay visible behind the window, too — the query at
     position i sees keys j <= i with j < sinks or j > i - window.  With ``sinks`` > 0 a gated result is rounded once, after
     the gate (otherwise also before it, as the reference does).
+    Rows of v that a window hides may be stale, but not infinite or NaN: near the keys that are seen they have weight 0.
     """
     return _native().sdpa_prefill(q, k, v, scale, mask_type, window, mask, gate, out, num_splits, return_lse, workspace,
                                   block_ids, block_ids_offset, out_copies, sinks)

@@ -117,7 +117,9 @@ typedef struct arc_sdpa_prefill_params {
     int32_t out_copy_count;
     /* The first `sinks` keys stay visible behind a window (optional, ARC_MASK_CAUSAL without block_ids): query at
      * position i sees keys j <= i with j < sinks or j > i - window.  0: none; without a window they change nothing.
-     * With sinks > 0 a gated result is rounded once, after the gate, and out_lse is that of the sums before any rounding. */
+     * With sinks > 0 a gated result is rounded once, after the gate, and out_lse is that of the sums before any rounding.
+     * As with a window alone, what is hidden from a query has weight 0 in its sum where another key of the same 128 is seen:
+     * rows of v between the sinks and the window may be stale, but not infinite or NaN (rows of k may be anything). */
     int32_t sinks;
 } arc_sdpa_prefill_params;
 
