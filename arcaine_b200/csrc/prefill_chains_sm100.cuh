@@ -516,6 +516,17 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
 
             // ---------------------------------------------------------- output: this warp's 32 rows, columns [64 s, 64 s + 64)
             const bool both = tw.blocks() > 1;  // (a single key block: B has none)
+            const int row0 = quarter * 32 + (lane >> 3), col = (lane & 7) * 8;  // this lane's first row, its columns of the warp's 64
+            const long long out0 = tw.b * p.o_stride_b + (tw.q0 + row0) * p.o_stride_t + (long long)tw.h * HD + s * 64 + col;
+            // (ONCE: the gate's values are asked for here, all at once, and come while the last products are waited for.  Asked for
+            // row by row behind them they were 3 us of latency: 2000 gated tokens of 28/4 heads, window 512, 55 -> 30 us.)
+            constexpr bool ONCE = GATE && SINKS;  // (an instance that never splits)
+            [[maybe_unused]] uint4 gates[ONCE ? 8 : 1];
+            if constexpr (ONCE) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    gates[i] = tw.q0 + row0 + 4 * i < p.seq ? *reinterpret_cast<const uint4*>(p.gate + out0 + 4 * i * p.o_stride_t) : make_uint4(0u, 0u, 0u, 0u);
+            }
             fin[s * 256 + r] = l;
             fin[s * 256 + 128 + r] = m;
             row_sync(quarter);
@@ -540,69 +551,87 @@ __global__ void __launch_bounds__(ChainsCfg::THREADS, 1)
             // could go.
             __syncwarp();  // (the tile before has left the buffer)
             const uint32_t at = smem_u32(out_buf) + lane * 128;
-            const int row0 = quarter * 32 + (lane >> 3), col = (lane & 7) * 8;  // this lane's first row, its columns of the warp's 64
-            const long long out0 = tw.b * p.o_stride_b + (tw.q0 + row0) * p.o_stride_t + (long long)tw.h * HD + s * 64 + col;
-            if (GATE && SINKS && !split) {  // the gate's values where the results go, for their rows' lanes
-                for (int i = 0; i < 8 && tw.q0 + row0 + 4 * i < p.seq; ++i) {
+            if constexpr (ONCE) {  // 16 columns a turn: gated in f32, over the gate's values in the buffer
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
                     const int rr = (lane >> 3) + 4 * i;
-                    *reinterpret_cast<uint4*>(out_buf + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)) = *reinterpret_cast<const uint4*>(p.gate + out0 + 4 * i * p.o_stride_t);
+                    *reinterpret_cast<uint4*>(out_buf + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)) = gates[i];
                 }
                 __syncwarp();
-            }
-            uint32_t a[32], b[32];
-            auto fetch = [&](int c) {
-                tmem_ld32(tO + s * 64 + c * 32, a);
-                if (both) tmem_ld32(tO + 128 + s * 64 + c * 32, b);
-            };
-            fetch(0);
+                uint32_t a[16], b[16];
+                auto fetch = [&](int c) {
+                    tmem_ld16(tO + s * 64 + c * 16, a);
+                    if (both) tmem_ld16(tO + 128 + s * 64 + c * 16, b);
+                };
+                fetch(0);
 #pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-                tmem_wait_ld();
-                float o[32];
+                for (int c = 0; c < 4; ++c) {
+                    tmem_wait_ld();
+                    float o[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const float x = __uint_as_float(a[e]) * fa;
-                    o[e] = both ? fmaf(__uint_as_float(b[e]), fb, x) : x;  // (nothing of B's: its columns may hold anything)
-                }
-                if (c == 0) {
-                    fetch(1);
-                } else {  // O is in registers: the next tile may overwrite the accumulators
-                    tc_fence_before_sync();
-                    mbar_arrive_warp(o_empty);
-                }
-                if (split) {
-                    if (store) {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + prow * HD + s * 64 + c * 32);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    for (int e = 0; e < 16; ++e) {
+                        const float x = __uint_as_float(a[e]) * fa;
+                        o[e] = both ? fmaf(__uint_as_float(b[e]), fb, x) : x;
                     }
-                    continue;
-                }
-                if constexpr (GATE && SINKS) {
-#pragma unroll 1
-                    for (int i = 0; i < 4; ++i) {
+                    if (c < 3) {
+                        fetch(c + 1);
+                    } else {
+                        tc_fence_before_sync();
+                        mbar_arrive_warp(o_empty);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t to = at + (((2 * c + i) ^ (lane & 7)) << 4);
                         uint32_t g[4];
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(g[0]), "=r"(g[1]), "=r"(g[2]), "=r"(g[3]) : "r"(at + (((4 * c + i) ^ (lane & 7)) << 4)));
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(g[0]), "=r"(g[1]), "=r"(g[2]), "=r"(g[3]) : "r"(to) : "memory");
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float gate = sigmoid(__uint_as_float(e & 1 ? g[e / 2] & 0xffff0000u : g[e / 2] << 16));
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (k == i) o[8 * k + e] *= gate;
-                        }
+                        for (int u = 0; u < 4; ++u)
+                            g[u] = pack_bf16x2(o[8 * i + 2 * u] * sigmoid(__uint_as_float(g[u] << 16)), o[8 * i + 2 * u + 1] * sigmoid(__uint_as_float(g[u] & 0xffff0000u)));
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(g[0]), "r"(g[1]), "r"(g[2]), "r"(g[3]) : "memory");
                     }
                 }
+            } else {
+                uint32_t a[32], b[32];
+                auto fetch = [&](int c) {
+                    tmem_ld32(tO + s * 64 + c * 32, a);
+                    if (both) tmem_ld32(tO + 128 + s * 64 + c * 32, b);
+                };
+                fetch(0);
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    tmem_wait_ld();
+                    float o[32];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((4 * c + i) ^ (lane & 7)) << 4)), "r"(pack_bf16x2(o[8 * i], o[8 * i + 1])),
-                                 "r"(pack_bf16x2(o[8 * i + 2], o[8 * i + 3])), "r"(pack_bf16x2(o[8 * i + 4], o[8 * i + 5])),
-                                 "r"(pack_bf16x2(o[8 * i + 6], o[8 * i + 7])) : "memory");
+                    for (int e = 0; e < 32; ++e) {
+                        const float x = __uint_as_float(a[e]) * fa;
+                        o[e] = both ? fmaf(__uint_as_float(b[e]), fb, x) : x;  // (nothing of B's: its columns may hold anything)
+                    }
+                    if (c == 0) {
+                        fetch(1);
+                    } else {  // O is in registers: the next tile may overwrite the accumulators
+                        tc_fence_before_sync();
+                        mbar_arrive_warp(o_empty);
+                    }
+                    if (split) {
+                        if (store) {
+                            float4* dst = reinterpret_cast<float4*>(p.part_o + prow * HD + s * 64 + c * 32);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                        continue;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((4 * c + i) ^ (lane & 7)) << 4)), "r"(pack_bf16x2(o[8 * i], o[8 * i + 1])),
+                                     "r"(pack_bf16x2(o[8 * i + 2], o[8 * i + 3])), "r"(pack_bf16x2(o[8 * i + 4], o[8 * i + 5])),
+                                     "r"(pack_bf16x2(o[8 * i + 6], o[8 * i + 7])) : "memory");
+                }
             }
             if (split) continue;
             __syncwarp();
             // (Gated two at a time: eight, 64 sigmoids of code that is fetched cold, cost a call of 100 rows 0.1 us less from warm caches
             // and 2.4 more from cold ones: 12.3 and 9.9.)
-            constexpr bool GATE_LATE = GATE && !SINKS;
+            constexpr bool GATE_LATE = GATE && !ONCE;
             constexpr int AT_ONCE = GATE_LATE ? 2 : 8;
 #pragma unroll AT_ONCE
             for (int i = 0; i < 8; ++i) {

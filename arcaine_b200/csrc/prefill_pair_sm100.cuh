@@ -338,13 +338,19 @@ __device__ __forceinline__ void stage_turn(const OutStage& s, const void* tm_out
         if (GATE)
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gw[4 * i]), "=r"(gw[4 * i + 1]), "=r"(gw[4 * i + 2]), "=r"(gw[4 * i + 3]) : "r"(at[i]));
     }
+    if constexpr (GATE && ONCE) {
+        float a[N];
 #pragma unroll
-    for (int u = 0; u < N / 2; ++u) {
-        float a0 = __uint_as_float(acc[2 * u]) * inv, a1 = __uint_as_float(acc[2 * u + 1]) * inv;
-        if constexpr (GATE && ONCE) a0 *= sigmoid(__uint_as_float(gw[u] << 16)), a1 *= sigmoid(__uint_as_float(gw[u] & 0xffff0000u));
-        w8[u] = pack_bf16x2(a0, a1);
+        for (int u = 0; u < N; ++u) a[u] = __uint_as_float(acc[u]) * inv;
+        taken();
+#pragma unroll
+        for (int u = 0; u < N / 2; ++u)
+            w8[u] = pack_bf16x2(a[2 * u] * sigmoid(__uint_as_float(gw[u] << 16)), a[2 * u + 1] * sigmoid(__uint_as_float(gw[u] & 0xffff0000u)));
+    } else {
+#pragma unroll
+        for (int u = 0; u < N / 2; ++u) w8[u] = pack_bf16x2(__uint_as_float(acc[2 * u]) * inv, __uint_as_float(acc[2 * u + 1]) * inv);
+        taken();
     }
-    taken();
 #pragma unroll
     for (int i = 0; i < N / 8; ++i) {
         if (GATE && !ONCE) {
