@@ -126,6 +126,28 @@ def test_sinks_strides_copies_and_aliases(hd, seq):
     assert torch.equal(q, out) and ops.device_status() == (0, 0)
 
 
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("seq,kv,nq,nkv", [(1, 130, 8, 4), (33, 33, 16, 1), (130, 400, 7, 7), (1100, 1100, 16, 8), (2300, 2300, 28, 4)])
+def test_sinks_gated_rows_of_a_wider_tensor(seq, kv, nq, nkv, hd):
+    """The gate and the output are parts of wider rows, and copies of the output go elsewhere; what lies beside them is left alone."""
+    from arcaine_b200 import ops
+    ops.clear_device_status()
+    q, k, v, _ = inputs(2, seq, kv, nq, nkv, hd, seed=seq)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    rows = 4 * torch.randn(2, seq, nq * hd + 16, generator=g, device=DEV).bfloat16()
+    wide, copy = torch.full_like(rows, 7.0), torch.full_like(rows, 5.0)
+    gate, out = (t[..., 8:8 + nq * hd].unflatten(-1, (nq, hd)) for t in (rows, wide))
+    addresses = torch.tensor([copy.data_ptr() + 16], dtype=torch.int64, device=DEV)  # (laid out like the output)
+    got, lse = ops.sdpa_prefill(q, k, v, scale=hd ** -0.5, mask_type=ops.MASK_CAUSAL, window=200, sinks=6, gate=gate, out=out, out_copies=addresses, return_lse=True)
+    assert ops.device_status() == (0, 0)
+    want, want_lse, size = plain(q, k, v, 200, 6, hd ** -0.5)
+    weight = torch.sigmoid(gate.double())
+    check(got, lse, want * weight, want_lse, size * weight)
+    assert bool((wide[..., :8] == 7.0).all()) and bool((wide[..., 8 + nq * hd:] == 7.0).all())
+    assert torch.equal(copy[..., 8:8 + nq * hd], wide[..., 8:8 + nq * hd])
+    assert bool((copy[..., :8] == 5.0).all()) and bool((copy[..., 8 + nq * hd:] == 5.0).all())
+
+
 FORCED = r"""
 import sys
 sys.path.insert(0, sys.argv[1] + '/tests')
