@@ -131,6 +131,8 @@ extern "C" int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void
     kp.weight[0] = static_cast<const uint16_t*>(p->q_weight);
     kp.weight[1] = static_cast<const uint16_t*>(p->k_weight);
     kp.fault = hs.fault;
+    static std::atomic<uint32_t> launches{0};
+    kp.own_fault = FAULT_BAD_KV_RANGE | launches.fetch_add(1, std::memory_order_relaxed) << FAULT_LAUNCH_SHIFT;
     kp.tokens = p->tokens;
     kp.page = pages ? p->page_size : 1;
     kp.num_rows = pages ? p->page_size * p->num_pages : 0;

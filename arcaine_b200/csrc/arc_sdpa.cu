@@ -1241,6 +1241,7 @@ extern "C" int arc_sdpa_device_status(uint32_t* fault_code, uint32_t* fault_deta
     uint32_t w[2] = {0, 0};
     if (cudaDeviceSynchronize() != cudaSuccess) return ARC_ERR_CUDA;
     if (cudaMemcpy(w, ds->fault, sizeof(w), cudaMemcpyDeviceToHost) != cudaSuccess) return ARC_ERR_CUDA;
+    w[0] &= (1u << FAULT_LAUNCH_SHIFT) - 1u;
     if (fault_code) *fault_code = w[0];
     if (fault_detail) *fault_detail = w[1];
     if (w[0] == 0) return ARC_OK;

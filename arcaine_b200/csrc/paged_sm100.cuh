@@ -144,6 +144,7 @@ struct QkvPagedParams {
     const double* inv_freq;
     const uint16_t* weight[2];
     uint32_t* fault;
+    uint32_t own_fault;          // what this launch reports a bad slot as (FAULT_LAUNCH_SHIFT)
     int tokens, page, num_rows;  // num_rows: of a pool
     int k0, v0, rows;            // a token's first K row, first V row, all its rows
     int half;                    // rotary_dim / 2
@@ -217,13 +218,16 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 3) qkv_prepare_paged_kernel(c
         begin_loads();
         fetch();
     }
-    if (__syncthreads_or(threadIdx.x == 0 && *reinterpret_cast<volatile uint32_t*>(p.fault) != 0u)) return;  // a status is set: no work
+    // A status is set: no work.  One of this launch's own, a bad slot that another CTA has met already, keeps nobody from the other tokens:
+    // CTAs start when there is room for them, beside other streams' kernels long after the first.
+    const uint32_t status = threadIdx.x == 0 ? *reinterpret_cast<volatile uint32_t*>(p.fault) : 0u;
+    if (__syncthreads_or(status != 0u && status != p.own_fault)) return;
 
     for (; left > 0; ++t, r0 = 0) {
         const int pos = f_pos;
         int slot = f_slot;
         if (slots && (slot >= p.num_rows || slot < -1)) {
-            if (lane == 0 && pos >= 0) report_fault(p.fault, FAULT_BAD_KV_RANGE, (uint32_t)t);
+            if (lane == 0 && pos >= 0) report_fault(p.fault, p.own_fault, (uint32_t)t);
             slot = -1;
         }
         const bool live = pos >= 0, stored = live && slot >= 0;  // (padding; rows that are not appended)

@@ -28,6 +28,9 @@ enum DeviceFault : uint32_t {
     FAULT_BAD_KV_RANGE = 10,  // not a wait: a sequence's rows, pages or slots reach past the cache, or its length past the stated bound
 };
 
+// Bits of a status word from here on may name the launch that reports it (0: any); the code is what is below.
+constexpr int FAULT_LAUNCH_SHIFT = 8;
+
 // First fault wins; `detail` says which iteration / barrier gave up.
 __device__ __forceinline__ void report_fault(uint32_t* fault, uint32_t code, uint32_t detail) {
     if (atomicCAS(fault, 0u, code) == 0u) fault[1] = detail;

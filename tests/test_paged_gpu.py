@@ -255,6 +255,52 @@ def test_prepare_bad_slots_are_not_written():
         ops.clear_device_status()
 
 
+@pytest.mark.parametrize("bad", [[0], [0, 12345, 29999]])
+def test_prepare_bad_slots_cost_no_other_token(bad):
+    """CTAs that start behind another stream's kernel find the status that a bad slot of their own call has set."""
+    from arcaine_b200 import ops
+    tokens, page = 30000, 16
+    q, k, v = (seeded_bf16(tokens, n, 128, seed=n).cuda() for n in (4, 2, 2))
+    positions, inv = torch.arange(tokens, dtype=torch.int32, device=DEV), ops.rope_frequencies(128, device=DEV)[0]
+    slots = torch.arange(tokens, dtype=torch.int32, device=DEV)
+    good = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    for t in bad:
+        slots[t], good[t] = 2**30 + t, False
+    want_q, want_k = q.clone(), k.clone()
+    ops.qkv_prepare_paged(want_q, want_k, None, positions, inv)
+    side, busy = torch.cuda.Stream(), seeded_bf16(8192, 8192, seed=9).cuda()
+
+    def call(got_q, kp, vp):
+        ops.qkv_prepare_paged(got_q, k, v, positions, inv, k_pages=kp, v_pages=vp, slots=slots)
+
+    for captured in (False, True):
+        got_q, kp, vp = q.clone(), *(torch.full((tokens // page + 1, page, 2, 128), 7.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                call(got_q, kp, vp)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.mm(busy, busy)
+        if captured:
+            graph.replay()
+        else:
+            call(got_q, kp, vp)
+        code, detail = ops.device_status()
+        assert code == 10 and detail in bad
+        assert torch.equal(got_q, want_q)
+        for pages, rows in ((kp, want_k), (vp, v)):
+            pages = pages.view(-1, 2, 128)
+            assert torch.equal(pages[:tokens][good], rows[good])
+            assert bool((pages[:tokens][~good] == 7.0).all()) and bool((pages[tokens:] == 7.0).all())
+        # a later call finds a status that is not its own: nothing is done
+        later = q.clone()
+        call(later, kp.fill_(5.0), vp.fill_(5.0))
+        assert torch.equal(later, q) and bool((kp == 5.0).all()) and bool((vp == 5.0).all())
+        assert ops.device_status() == (code, detail)
+        ops.clear_device_status()
+
+
 def test_prepare_refusals():
     from arcaine_b200 import ops
     q, k = seeded_bf16(4, 4, 128, seed=1).cuda(), seeded_bf16(4, 2, 128, seed=2).cuda()
