@@ -909,7 +909,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, XCHG || COLS < 256 ? 1 : 4) sdp
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-            inv = 1.f / z;
+            inv = PAGED && z == 0.f ? 0.f : 1.f / z;  // (PAGED: all scores -inf give zeros, as no keys do)
             lse = mx + __logf(z);
         }
     }

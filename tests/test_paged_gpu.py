@@ -514,6 +514,30 @@ def test_decode_infinite_and_missing_numbers_stay_in_their_row():
             assert torch.equal(out[keep], w[keep]) and bool(torch.isfinite(lse[keep]).all())
 
 
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("batch,nq,nkv,ctas,n", [(2, 4, 2, 0, 300), (130, 8, 2, 0, 100), (1, 2, 1, 148, 300), (20, 8, 2, 148, 300), (200, 8, 2, 148, 100)])
+@pytest.mark.parametrize("value,factor", [(-math.inf, 1.0), (-1e38, 100.0)])
+def test_decode_scores_of_minus_infinity(hd, batch, nq, nkv, ctas, n, value, factor):
+    """Keys whose scores are all -inf, or pass fp32: zeros and a log-sum-exp of -inf, as without keys, in one launch and behind each merge.  The
+    first sequence has one key with a score of its own, which takes all the weight."""
+    from arcaine_b200 import ops
+    page = 16
+    width = -(-n // page)
+    table = torch.arange(batch * width, dtype=torch.int32, device=DEV).view(batch, width)
+    kp = torch.full((batch * width, page, nkv, hd), value, dtype=torch.bfloat16, device=DEV)
+    vp = seeded_bf16(batch * width, page, nkv, hd, seed=hd).cuda()
+    q = ((1 + seeded_bf16(batch, nq, hd, seed=2).float().abs()) * factor).bfloat16().cuda()
+    for one in (False, True):
+        if one:
+            kp[width - 1, 0] = 0.5
+        out, o32, lse = ops.sdpa_decode_paged(q, kp, vp, table, ints([n] * batch), scale=0.1, return_partial=True, num_ctas=ctas)
+        assert bool((out[int(one):] == 0).all()) and bool((o32[int(one):] == 0).all()) and bool((lse[int(one):] == -math.inf).all())
+        if one:
+            seen = vp[width - 1, 0].repeat_interleave(nq // nkv, 0)
+            assert torch.equal(out[0], seen) and bool(torch.isfinite(lse[0]).all())
+    assert ops.device_status() == (0, 0)
+
+
 def test_decode_large_scores():
     """One key takes all the weight, and scores of some thousand neither overflow nor lose the others' rows."""
     from arcaine_b200 import ops
