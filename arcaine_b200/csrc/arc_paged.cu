@@ -70,6 +70,7 @@ extern "C" int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void
     if (p->tokens < 0 || (p->q && p->nq < 1) || (p->k && p->nkv < 1)) return ARC_ERR_BAD_SHAPE;
     if (p->rotary_dim < 0 || p->rotary_dim > p->hd || p->rotary_dim % 16 != 0) return ARC_ERR_BAD_SHAPE;
     if (!std::isfinite(p->eps) || p->eps < 0.f || !std::isfinite(p->mscale)) return ARC_ERR_BAD_SHAPE;
+    if (p->tokens == 0) return ARC_OK;  // (ahead of the pointers: an empty tensor has none)
     if (p->v && !p->k) return ARC_ERR_NULL_POINTER;
     if ((p->q && !p->q_out) || (p->k && !p->k_out && !p->k_pages) || (p->v && !p->v_out && !p->v_pages)) return ARC_ERR_NULL_POINTER;
     if ((p->rotary_dim > 0 && !p->inv_freq) || !p->positions) return ARC_ERR_NULL_POINTER;
@@ -97,7 +98,6 @@ extern "C" int arc_qkv_prepare_paged(const arc_qkv_prepare_paged_params* p, void
         if (p->k_pages && (rc = check_pool(p->k_stride_page, p->k_stride_t, p->page_size, p->num_pages, row)) != ARC_OK) return rc;
         if (p->v && p->v_pages && (rc = check_pool(p->v_stride_page, p->v_stride_t, p->page_size, p->num_pages, row)) != ARC_OK) return rc;
     }
-    if (p->tokens == 0) return ARC_OK;
     HostState hs;
     if ((rc = host_state(&hs)) != ARC_OK) return rc;
 

@@ -361,6 +361,7 @@ int arc_paged_tables(const arc_paged_tables_params* p, void* stream);
  * A slot of num_pages * page_size or more (or below -1) is not written and shows as ARC_ERR_DEVICE_BAD_RANGE in
  * arc_sdpa_device_status() (detail: the token); the call's other tokens are worked on as ever, later calls' not.  (The replays of a
  * captured call are one call in this.)  Slots of a call must differ.  q, k and v may each be NULL; v needs k.
+ * Without tokens nothing is done, whatever the pointers.
  * hd in {128, 256, 512}; rotary_dim a multiple of 16, <= hd; strides in elements, multiples of 8; pointers 16-byte aligned. */
 typedef struct arc_qkv_prepare_paged_params {
     const void* q;  /* (tokens, nq, hd) bf16, or NULL */

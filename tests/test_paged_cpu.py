@@ -102,6 +102,15 @@ def test_prepare_refusals():
     assert call(tokens=0) == _lib.ARC_OK
 
 
+def test_prepare_of_no_tokens_needs_no_addresses():
+    """A step without tokens: empty tensors have no address."""
+    from arcaine_b200 import _lib
+    p = _lib.QkvPreparePagedParams(tokens=0, nq=2, nkv=1, hd=128, page_size=16, num_pages=4, rotary_dim=128, norm_qk=1, eps=1e-6, mscale=1.0)
+    assert _lib.load().arc_qkv_prepare_paged(ctypes.byref(p), None) == _lib.ARC_OK
+    p.rotary_dim = 24
+    assert _lib.load().arc_qkv_prepare_paged(ctypes.byref(p), None) == _lib.ARC_ERR_BAD_SHAPE
+
+
 def test_decode_refusals():
     from arcaine_b200 import _lib
     lib, m = _lib.load(), Memory()

@@ -301,6 +301,19 @@ def test_prepare_bad_slots_cost_no_other_token(bad):
         ops.clear_device_status()
 
 
+def test_a_step_of_no_tokens():
+    from arcaine_b200 import ops
+    table = torch.zeros(2, 2, dtype=torch.int32, device=DEV)
+    slots, positions, begin, kv_len, used = ops.paged_tables(ints([0, 0]), ints([3, 0]), table, ints([]), page_size=16, num_tokens=0)
+    assert slots.shape == positions.shape == (0,) and begin.tolist() == [0, 0, 0] and kv_len.tolist() == [3, 0] and used.tolist() == [0]
+    q, k = (torch.empty(0, n, 128, dtype=torch.bfloat16, device=DEV) for n in (4, 2))
+    pages = torch.full((2, 16, 2, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    launches = ops.launch_count()
+    ops.qkv_prepare_paged(q, k, k, positions, ops.rope_frequencies(128, device=DEV)[0], k_pages=pages, v_pages=pages, slots=slots)
+    ops.qkv_prepare_paged(q, None, None, positions, None, q_out=q.clone())
+    assert ops.launch_count() == launches and bool((pages == 7.0).all()) and ops.device_status() == (0, 0)
+
+
 def test_prepare_refusals():
     from arcaine_b200 import ops
     q, k = seeded_bf16(4, 4, 128, seed=1).cuda(), seeded_bf16(4, 2, 128, seed=2).cuda()
