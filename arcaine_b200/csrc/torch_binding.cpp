@@ -700,7 +700,7 @@ T* vector_of(PyObject* o, c10::ScalarType type, int64_t n, bool exactly, const T
 const Tensor& table_of(PyObject* o, const Tensor& ref, int64_t batch) {
     const Tensor& t = need_tensor(o, at::kInt, "block_table");
     same_device(t, ref, "block_table");
-    if (t.dim() != 2 || t.size(0) != batch || t.size(1) < 1 || t.stride(1) != 1 || (batch > 1 && t.stride(0) < t.size(1)))
+    if (t.dim() != 2 || t.size(0) != batch || t.size(1) < 1 || (t.size(1) > 1 && t.stride(1) != 1) || (batch > 1 && t.stride(0) < t.size(1)))
         bad("block_table must be (batch, width) int32 with contiguous rows that do not overlap");
     return t;
 }

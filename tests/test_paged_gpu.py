@@ -510,6 +510,24 @@ def test_views_of_one_head_or_one_token():
     assert ops.device_status() == (0, 0) and torch.equal(out, want)
 
 
+def test_tables_of_one_column_out_of_a_transposed_list():
+    """(B, 1) with a stride of B behind the last dimension, which has one element."""
+    from arcaine_b200 import ops
+    pages, q = seeded_bf16(5, 16, 2, 128, seed=3).cuda(), seeded_bf16(3, 4, 128, seed=4).cuda()
+    table = ints([[4, 0, 2]]).t()
+    assert table.stride() == (1, 3)
+    lens = ints([16, 1, 9])
+    got = ops.sdpa_decode_paged(q, pages, pages, table, lens, scale=0.1)
+    assert torch.equal(got, ops.sdpa_decode_paged(q, pages, pages, table.clone(memory_format=torch.contiguous_format), lens, scale=0.1))
+    new, past, table = ints([1, 2, 0]), ints([3, 0, 0]), ints([[4, -7, -7]]).t()
+    step = ops.paged_tables(new, past, table, ints([1, 3]), page_size=16, num_tokens=3)
+    want = plain_tables([1, 2, 0], [3, 0, 0], [[4], [-7], [-7]], [1, 3], 16, 3)
+    assert [t.tolist() for t in step] == list(want[:5]) and table.tolist() == want[5]
+    with pytest.raises(ValueError, match="block_table"):  # rows in one place
+        ops.sdpa_decode_paged(q, pages, pages, ints([[0]]).expand(3, 1), lens, scale=0.1)
+    assert ops.device_status() == (0, 0)
+
+
 def test_decode_infinite_and_missing_numbers_stay_in_their_row():
     from arcaine_b200 import ops
     lens = [700, 700, 700]
