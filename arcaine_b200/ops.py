@@ -361,9 +361,10 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: Option
 
     ``scaling``, for contexts ``factor`` times as long as ``original_len``, which the model was trained on: None; ``"linear"``
     (positions divided by the factor); ``"ntk"`` (theta times factor^(d / (d - 2)): the slowest pair turns ``factor`` times
-    slower, the fastest as before); ``"yarn"`` (arXiv:2309.00071: pairs that turn less than ``beta_slow`` times over
-    ``original_len`` are divided by the factor, those over ``beta_fast`` times are left, a ramp between; mscale =
-    0.1 ln(factor) + 1)."""
+    slower, the fastest as before); ``"yarn"`` (arXiv:2309.00071, with the ramp that checkpoints of that type are run with: linear in the
+    pair's index, from the last pair that turns ``beta_fast`` times over ``original_len`` (its index rounded down), which is left as it
+    is, to the first that turns ``beta_slow`` times (rounded up), which is divided by the factor.  The paper's own text has a ramp in
+    the number of turns, whose frequencies differ by up to 2.3 times in between.  mscale = 0.1 ln(factor) + 1)."""
     if rotary_dim <= 0 or rotary_dim % 16 != 0:
         raise ValueError("rotary_dim must be a positive multiple of 16")
     if not theta > 0.0 or not math.isfinite(theta):
@@ -378,13 +379,15 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: Option
     if scaling == "linear":
         inv = [w / factor for w in inv]
     if scaling == "yarn":
-        if original_len <= 0 or not beta_fast > beta_slow:
-            raise ValueError("yarn needs original_len and beta_fast > beta_slow")
+        if original_len <= 0 or not beta_fast > beta_slow > 0.0 or not theta > 1.0:
+            raise ValueError("yarn needs original_len, beta_fast > beta_slow > 0 and theta > 1")
 
-        def kept(w):
-            return min(1.0, max(0.0, (original_len * w / (2 * math.pi) - beta_slow) / (beta_fast - beta_slow)))
+        def turning(times):  # the index, not a whole one, of the pair that turns so often over original_len
+            return rotary_dim * math.log(original_len / (2 * math.pi * times)) / (2 * math.log(theta))
 
-        inv = [w * kept(w) + w / factor * (1.0 - kept(w)) for w in inv]
+        low, high = max(math.floor(turning(beta_fast)), 0), min(math.ceil(turning(beta_slow)), rotary_dim - 1)
+        kept = [min(1.0, max(0.0, (high - f) / (high - low))) if high > low else float(f <= low) for f in range(rotary_dim // 2)]
+        inv = [w * k + w / factor * (1.0 - k) for w, k in zip(inv, kept)]
         mscale = 0.1 * math.log(factor) + 1.0
     return torch.tensor(inv, dtype=torch.float64, device=device), mscale
 

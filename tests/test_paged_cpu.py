@@ -172,3 +172,31 @@ def test_rope_frequencies():
                dict(rotary_dim=64, scaling="linear", factor=0.5), dict(rotary_dim=64, scaling="yarn", factor=2.0)):
         with pytest.raises(ValueError):
             ops.rope_frequencies(**kw, device="cpu")
+
+
+@pytest.mark.parametrize("theta,length,factor,low,high", [(1e6, 32768, 4.0, 23, 40), (1e4, 4096, 8.0, 20, 46), (1e6, 8192, 8.0, 17, 34)])
+def test_yarn_ramp_goes_by_the_index_of_the_pair(theta, length, factor, low, high):
+    """Of 64 pairs: up to `low` as they are, from `high` on divided, linear in the index between them.  low and high are worked out by hand:
+    pair f turns length theta^(-f / 64) / (2 pi) times, so that the ends are the last whole f with 32 turns or more and the first with
+    one or less."""
+    from arcaine_b200 import ops
+    turns = [length * theta ** (-f / 64) / (2 * math.pi) for f in range(64)]
+    assert turns[low] >= 32 > turns[low + 1] and turns[high] <= 1 < turns[high - 1]
+    inv = ops.rope_frequencies(128, theta, device="cpu")[0]
+    got, m = ops.rope_frequencies(128, theta, scaling="yarn", factor=factor, original_len=length, device="cpu")
+    assert math.isclose(m, 0.1 * math.log(factor) + 1.0)
+    for f in range(64):
+        share = min(1.0, max(0.0, (f - low) / (high - low)))  # of the divided frequency
+        assert math.isclose(got[f].item(), inv[f].item() * (1.0 - share + share / factor), rel_tol=1e-12), f
+
+
+def test_yarn_ends_outside_the_pairs():
+    from arcaine_b200 import ops
+    inv = ops.rope_frequencies(32, 1e4, device="cpu")[0]
+    # the fastest pair turns 16 times: the ramp begins with it; the slowest 10^5 times: all are left
+    got = ops.rope_frequencies(32, 1e4, scaling="yarn", factor=4.0, original_len=101, device="cpu")[0]
+    assert got[0] == inv[0] and bool((got[1:] < inv[1:]).all())
+    assert torch.equal(ops.rope_frequencies(32, 1e4, scaling="yarn", factor=4.0, original_len=2**31 - 1, beta_fast=64.0, beta_slow=32.0, device="cpu")[0], inv)
+    for kw in (dict(theta=1.0), dict(theta=0.5), dict(beta_slow=0.0), dict(beta_slow=-1.0), dict(beta_fast=1.0), dict(beta_slow=math.nan)):
+        with pytest.raises(ValueError, match="yarn needs"):
+            ops.rope_frequencies(64, **{"theta": 1e4, **kw}, scaling="yarn", factor=2.0, original_len=4096, device="cpu")
