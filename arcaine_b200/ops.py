@@ -403,7 +403,8 @@ def qkv_prepare_paged(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: O
 
     q (T, nq, hd), k, v (T, nkv, hd); ``positions`` (T,) int32; ``inv_freq`` float64 (rotary_dim / 2,) on the device and ``mscale`` as
     :func:`rope_frequencies` gives them (None: no rotation).  Pairs are (f, f + rotary_dim / 2), or (2 f, 2 f + 1) with
-    ``interleaved``; rotary_dim a multiple of 16, the rest of the head is not rotated.  Angles are exact at any position.
+    ``interleaved``; rotary_dim a multiple of 16, the rest of the head is not rotated.  Angles are worked out in
+    64 bits: less than 1e-6 rad off at any position, for frequencies of at most 1.
     Norm and rotation are in fp32 and rounded once (:func:`qkv_prepare` rounds between them, as the reference does).
     ``norm=False`` rotates only; ``v_norm`` gives V rows a unit-RMS norm.
 

@@ -355,7 +355,8 @@ int arc_paged_tables(const arc_paged_tables_params* p, void* stream);
  *   y = x * rsqrt(mean(x^2) + eps) * weight     Q and K rows if norm_qk (weight NULL: 1), V rows if norm_v (no weight)
  *   Q and K rows, pairs f < rotary_dim / 2:  (y[a], y[b]) = (y[a] c - y[b] s, y[a] s + y[b] c)
  *     a, b = f, f + rotary_dim / 2 (half layout) or 2 f, 2 f + 1 (interleaved);
- *     c, s = mscale * cos, sin(positions[token] * inv_freq[f]), the angle in 64 bits: exact however far the position.
+ *     c, s = mscale * cos, sin(positions[token] * inv_freq[f]), the angle in 64 bits: off by 3 * 2^-53 of
+ *     itself and 1e-7 rad at most, so by less than 1e-6 rad at any position that 31 bits hold while inv_freq <= 1.
  * Q rows go to q_out (may be q).  K and V rows go to row slots[token] of the pages (a slot of -1: nowhere) and, if given,
  * to k_out / v_out (may be k / v).  A token with a negative position is padding: nothing of it is read or written.
  * A slot of num_pages * page_size or more (or below -1) is not written and shows as ARC_ERR_DEVICE_BAD_RANGE in

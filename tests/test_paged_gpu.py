@@ -230,6 +230,29 @@ def test_prepare(tokens, nq, nkv, hd, rotary, interleaved, norm, v_norm, weights
     assert torch.equal(fused[:, -8:], before[:, -8:])
 
 
+def test_prepare_angles_of_far_positions():
+    """Positions close to multiples of pi, the numerators of its convergents among them: the sine is small, and bf16 shows the angle to 2^-8 of
+    it.  A position may be off by 1e-6 rad: three roundings to 64 bits, 3 * 2^-53 * 2^31 = 7.2e-7, and one to fp32, 2 pi 2^-26 = 9.4e-8."""
+    from decimal import Decimal, getcontext
+
+    from arcaine_b200 import ops
+    getcontext().prec = 60
+    pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+    far = [355, 103993, 80143857, 165707065, 245850922, 411557987, 1068966896, 2 * 1068966896, 2**31 - 1, 2**31 - 2, 1068966896 + 355, 1068966896 + 103993]
+    far += [int(round(pi * n)) for n in range(650000000, 683000000, 1999999)]
+    x = torch.zeros(len(far), 1, 128, dtype=torch.bfloat16, device=DEV)
+    x[..., 0] = 1.0
+    inv = torch.zeros(8, dtype=torch.float64, device=DEV)
+    inv[0] = 1.0
+    ops.qkv_prepare_paged(x, None, None, ints(far), inv, norm=False)
+    for at, c, s in zip(far, x[:, 0, 0].tolist(), x[:, 0, 8].tolist()):
+        half_turns = int((Decimal(at) / pi).to_integral_value())
+        rest = float(Decimal(at) - pi * half_turns)
+        want = math.sin(rest) * (-1) ** half_turns, math.cos(rest) * (-1) ** half_turns
+        assert abs(s - want[0]) <= 1e-6 + 2.0 ** -8 * abs(want[0]), at
+        assert abs(c - want[1]) <= 1e-6 + 2.0 ** -8 * abs(want[1]), at
+
+
 def test_prepare_only_queries_or_only_keys():
     from arcaine_b200 import ops
     q, k = seeded_bf16(9, 4, 128, seed=1).cuda(), seeded_bf16(9, 2, 128, seed=2).cuda()
