@@ -410,8 +410,8 @@ def qkv_prepare_paged(q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: O
 
     Q is rewritten in place or goes to ``q_out``.  K and V go to rows ``slots`` (T,) of ``k_pages`` / ``v_pages`` (num_pages,
     page_size, nkv, hd), and to ``k_out`` / ``v_out`` if given (which may be k and v: a prompt's attention reads them there);
-    without pages they are rewritten in place.  A slot of -1 is not appended; a token with a negative position is padding,
-    of which nothing is read or written.  Slots of a call must differ; one outside the pool is not written and shows in
+    without pages they are rewritten in place.  A slot of -1 is not appended; a token with a negative position is padding:
+    its rows may hold anything and nothing of it is written.  Slots of a call must differ; one outside the pool is not written and shows in
     ``device_status()`` (``FAULT_BAD_KV_RANGE``; detail: the token), which leaves the call's other tokens as they should be.
     """
     _native().qkv_prepare_paged(q, k, v, positions, inv_freq, k_pages, v_pages, slots, norm, v_norm, q_weight, k_weight, eps,

@@ -19,6 +19,10 @@
  *   - score = (q . k) * scale + mask, softmax in fp32
  *     (src/common/layers/attention_batched.hpp:28-44).
  *   - `stream` is a cudaStream_t passed as void*.
+ *   - Parameter structs are cleared before they are filled (`= {0}`): 0 is every
+ *     optional field's "not used".  A program is rebuilt with the header of its
+ *     library: new fields come behind the others, also where padding was
+ *     (`sinks` of arc_sdpa_prefill_params).
  */
 #ifndef ARC_SDPA_H_
 #define ARC_SDPA_H_
@@ -331,7 +335,7 @@ int arc_qkv_prepare(const arc_qkv_prepare_params* p, void* stream);
  * are -1 (padding that arc_qkv_prepare_paged passes over), so that a captured step may bring fewer tokens.
  * A negative length, one that does not fit the table's row (or 31 bits), or more than num_tokens tokens: nothing is written, and
  * arc_sdpa_device_status() shows ARC_ERR_DEVICE_BAD_RANGE (detail: the request; batch where the sum is too large).
- * batch <= 2048, num_tokens <= 2^30.  kv_len must not overlap past_len.  4-byte alignment is enough. */
+ * batch <= 2048, num_tokens <= 2^30.  What is written must not overlap what is read (the table apart).  4-byte alignment is enough. */
 typedef struct arc_paged_tables_params {
     const int32_t* new_len;    /* [batch] */
     const int32_t* past_len;   /* [batch] or NULL */
@@ -358,7 +362,8 @@ int arc_paged_tables(const arc_paged_tables_params* p, void* stream);
  *     c, s = mscale * cos, sin(positions[token] * inv_freq[f]), the angle in 64 bits: off by 3 * 2^-53 of
  *     itself and 1e-7 rad at most, so by less than 1e-6 rad at any position that 31 bits hold while inv_freq <= 1.
  * Q rows go to q_out (may be q).  K and V rows go to row slots[token] of the pages (a slot of -1: nowhere) and, if given,
- * to k_out / v_out (may be k / v).  A token with a negative position is padding: nothing of it is read or written.
+ * to k_out / v_out (may be k / v).  A token with a negative position is padding: nothing of it is written.
+ * Its rows may hold anything, but are read like all others: memory must be behind them.
  * A slot of num_pages * page_size or more (or below -1) is not written and shows as ARC_ERR_DEVICE_BAD_RANGE in
  * arc_sdpa_device_status() (detail: the token); the call's other tokens are worked on as ever, later calls' not.  (The replays of a
  * captured call are one call in this.)  Slots of a call must differ.  q, k and v may each be NULL; v needs k.
@@ -468,8 +473,8 @@ int arc_sdpa_allgather_merge(const float* record, float* gathered, int32_t world
 
 /* Device-side status of the current device: ARC_OK, ARC_ERR_DEVICE_WAIT_TIMEOUT (the first bounded
  * wait that gave up since the last clear; fault_code says which kind, fault_detail where) or
- * ARC_ERR_DEVICE_BAD_RANGE (fault_detail = the sequence).  While a status is set, launches
- * return at once without doing their work.  Synchronises the device. */
+ * ARC_ERR_DEVICE_BAD_RANGE (fault_detail = the sequence, request or token).  While a status is set,
+ * launches return at once without doing their work.  Synchronises the device. */
 int arc_sdpa_device_status(uint32_t* fault_code, uint32_t* fault_detail);
 int arc_sdpa_clear_device_status(void);
 
