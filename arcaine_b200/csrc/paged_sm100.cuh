@@ -144,7 +144,6 @@ struct QkvPagedParams {
     const double* inv_freq;
     const uint16_t* weight[2];
     uint32_t* fault;
-    uint32_t own_fault;          // what this launch reports a bad slot as (FAULT_LAUNCH_SHIFT)
     int tokens, page, num_rows;  // num_rows: of a pool
     int k0, v0, rows;            // a token's first K row, first V row, all its rows
     int half;                    // rotary_dim / 2
@@ -152,6 +151,7 @@ struct QkvPagedParams {
     long long q_stride, k_stride, v_stride, q_dst_stride, k_also_stride, v_also_stride;
     long long k_page_stride, v_page_stride, k_row_stride, v_row_stride;  // row stride: between two rows of a page, or two tokens
     float eps, mscale;
+    uint32_t own_fault;          // what this launch reports a bad slot as (FAULT_LAUNCH_SHIFT)
 };
 
 // A pass is 512 / HD rows of a token by a warp.  All tokens' passes are laid end to end and cut into equal parts, one per warp, which may
@@ -220,8 +220,9 @@ __global__ void __launch_bounds__(32 * PREP_WARPS, 3) qkv_prepare_paged_kernel(c
     }
     // A status is set: no work.  One of this launch's own, a bad slot that another CTA has met already, keeps nobody from the other tokens:
     // CTAs start when there is room for them, beside other streams' kernels long after the first.
-    const uint32_t status = threadIdx.x == 0 ? *reinterpret_cast<volatile uint32_t*>(p.fault) : 0u;
-    if (__syncthreads_or(status != 0u && status != p.own_fault)) return;
+    // (A status stays as it is while kernels run, so that all threads find the same one.)
+    const auto status = [&] { return *reinterpret_cast<volatile uint32_t*>(p.fault); };
+    if (__syncthreads_or(threadIdx.x == 0 && status() != 0u) && status() != p.own_fault) return;
 
     for (; left > 0; ++t, r0 = 0) {
         const int pos = f_pos;
