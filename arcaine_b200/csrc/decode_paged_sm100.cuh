@@ -12,7 +12,8 @@
 // Bound by HBM where there is much to read: 64 sequences of 1 K to 32 K keys, 24/4 heads of 256, 3.07 GB, 455 us (6.75 TB/s, of a copy's
 // 6.54); 48 streams of 300 to 65536 keys behind a window of 1024 with 4 sinks, 28/4 of 128, 88 MB, 21.9 (13.5 at the copy rate).
 // Where there is little, by a chain of latencies: one token of 24/4 heads of 256 over 513 keys 6.2.  A CTA on its own streams what its copies
-// let it: 63 GB/s by 4 KB (one head of 128 a slice), 77 by 8, 85 by 16, and without the arithmetic 80, 98, 110.
+// let it.  One by shares, the others idle: with 1 / 2 / 4 / 8 heads of 128 a copy (4 to 32 KB) 56 / 71 / 78 / 88 GB/s, with 1 / 2 / 4 of
+// 256 78 / 84 / 94.  That of one long sequence in clusters of one, beside short ones: 61 with a head of 128, 83 with two, 77 with one of 256.
 #pragma once
 #include "decode_sm100.cuh"
 
