@@ -193,8 +193,7 @@ static int paged_slices(int hd, int heads, int subs) { return std::max(1, std::m
 // One launch or two?  Clusters take 4.8 us and the longer of two times: of a CTA of the longest sequence, taken to stream 65 / 70 / 85 GB/s with
 // one / two / four and more KV heads of 128 and 91 with heads of 256 (measured rates: decode_paged_sm100.cuh; one of 1200 keys
 // among 19 of 16, a head each 14.0 us where this says 14.2; among 59, two heads each 18.9 and 22.4; of 900, heads of 256 16.5 and 15.1), and of
-// all keys at 6.5 TB/s.  Shares read those at the same
-// rate, whatever the lengths, but cost 7 us, up to 3 more that parts of a few slices do not hide, and 0.03 for each sequence (the
+// all keys at 6.5 TB/s.  Shares read those at the same rate, whatever the lengths, but cost 7 us, up to 3 more that parts of a few slices do not hide, and 0.03 for each sequence (the
 // second launch, the records, shares that two sequences divide).  (us, shares and clusters, all sequences as long: one token of 24/4
 // heads of 256 over 513 keys 7.2 and 6.1, of 28/4 of 128 over 4100 10.6 and 9.2; 16 over 1028 15.5 and 11.1; 48 26.9 and 22.2; 100
 // 43.2 and 39.2; 128 of 16/2 over 4100 94 and 83.)  Lengths on the device are not known here, only what a table row can name and what

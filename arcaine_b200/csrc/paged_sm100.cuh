@@ -161,7 +161,8 @@ struct QkvPagedParams {
 // l + HD / 16, each with its own four pairs.  Norm and rotation stay in fp32 and are rounded once.
 //
 // Angles: turns = position * inv_freq / 2 pi in 64 bits (three roundings: 3 * 2^-53 of them, 1.2e-7 turns at position 2^31 and one
-// radian each), less the nearest whole number; what is left, at most half a turn, is rounded to fp32 (2^-26 turns) and goes to sincospif.  (In fp32 the angle of position 500000 would be off by 0.03 rad.)  Once a token and pair, not a head.
+// radian each), less the nearest whole number; what is left, at most half a turn, is rounded to fp32 (2^-26 turns) and goes to
+// sincospif.  (In fp32 the angle of position 500000 would be off by 0.03 rad.)  Once a token and pair, not a head.
 //
 // Bound by HBM, reads and writes mixed; a pass's rows are asked for one ahead, over the end of a token, too, and with them the
 // next token's position and slot.  (16384 tokens of 32/16 heads of 128, 537 MB: 149 us asked for when needed, two CTAs an SM; 100 a
